@@ -20,8 +20,9 @@ CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "_r2d2dpg_hip.so")
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 
-HIP_SOURCES = ["lstm.hip", "lstm_px.hip", "td_polyak.hip", "sumtree.hip", "replay_pack.hip"]
-CPP_SOURCES = ["bindings.cpp"]
+HIP_SOURCES = ["lstm.hip", "lstm_px.hip", "td_polyak.hip", "sumtree.hip", "replay_pack.hip",
+               "layer_norm.hip", "gated_recurrence.hip", "gated_linear.hip"]
+CPP_SOURCES = ["bindings.cpp", "bindings_gated.cpp"]
 
 
 def _run(cmd):
@@ -33,7 +34,7 @@ def _newer(src, obj):
     if not os.path.exists(obj):
         return True
     st = os.path.getmtime
-    deps = [src, os.path.join(CSRC, "common.h")]
+    deps = [src] + [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
     return any(st(d) > st(obj) for d in deps if os.path.exists(d))
 
 

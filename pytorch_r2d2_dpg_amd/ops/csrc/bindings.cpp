@@ -652,7 +652,10 @@ torch::Tensor fp8_gather_decode(torch::Tensor store, torch::Tensor idx,
 
 }  // namespace
 
+void bind_gated(py::module_& m);  // bindings_gated.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    bind_gated(m);
     m.def("lstm_seq_fwd", &lstm_seq_fwd, "fused LSTM sequence forward (K1)",
           py::arg("gates_x"), py::arg("h0"), py::arg("c0"), py::arg("wh"),
           py::arg("stash") = true);

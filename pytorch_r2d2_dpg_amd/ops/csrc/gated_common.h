@@ -1,0 +1,97 @@
+// Shared by the layer norm, gated recurrence and gated linear kernels.
+#pragma once
+
+#include "common.h"
+
+#include <cstdint>
+
+using bf16 = __hip_bfloat16;
+
+DEV_INLINE float to_f(float v) { return v; }
+DEV_INLINE float to_f(bf16 v) { return bf2f(v); }
+template <typename E> DEV_INLINE E from_f(float v);
+template <> DEV_INLINE float from_f<float>(float v) { return v; }
+template <> DEV_INLINE bf16 from_f<bf16>(float v) { return f2bf(v); }
+
+// sigma(x) and sigma(-x) = 1 - sigma(x) from one exponential of -|x|: neither
+// cancels where the other is near one. The exp2 and rcp instructions are within
+// 1 ulp, the argument's rounding adds |x| * 2^-24.
+DEV_INLINE void sigmoid_pair(float x, float& pos, float& neg) {
+    const float e = __builtin_amdgcn_exp2f(-fabsf(x) * 1.44269504f);
+    const float big = __builtin_amdgcn_rcpf(1.0f + e);
+    const float small = e * big;
+    pos = x >= 0.0f ? big : small;
+    neg = x >= 0.0f ? small : big;
+    if (x != x) pos = neg = x;
+}
+
+// silu(x) = x * sigma(x) and its derivative sigma + x sigma (1 - sigma).
+DEV_INLINE void silu_grad(float x, float& val, float& grad) {
+    float s, n;
+    sigmoid_pair(x, s, n);
+    val = x * s;
+    grad = s * (1.0f + x * n);
+}
+
+// N consecutive elements in one memory instruction, whatever their alignment
+// (global loads and stores need none beyond the element's on this target).
+template <typename E, int N>
+struct __attribute__((packed, aligned(sizeof(E)))) Run {
+    E v[N];
+};
+
+// Elements p[0..N) of which the first `have` exist; the others read as 0.
+template <typename E, int N>
+DEV_INLINE void load_run(const E* p, int have, E (&out)[N]) {
+    if (have >= N) {
+        const Run<E, N> r = *reinterpret_cast<const Run<E, N>*>(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = r.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = i < have ? p[i] : from_f<E>(0.0f);
+    }
+}
+
+template <typename E, int N>
+DEV_INLINE void store_run(E* p, int have, const E (&in)[N]) {
+    if (have >= N) {
+        Run<E, N> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] = in[i];
+        *reinterpret_cast<Run<E, N>*>(p) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < have) p[i] = in[i];
+    }
+}
+
+DEV_INLINE float wave_sum(float v) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+
+// out[c] = sum over r of part[r][c], rows in a fixed order: the second stage of
+// a reduction over rows, in place of atomics whose order would change results.
+// 16 waves share 64 columns, wave w the rows w, w+16, ...
+template <typename E>
+__global__ void __launch_bounds__(1024)
+column_sum_kernel(const float* __restrict__ part, E* __restrict__ out,
+                  int rows, int cols) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (c < cols)
+        for (int r = wave; r < rows; r += 16) s += part[(int64_t)r * cols + c];
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < cols) {
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) t += sums[w][lane];
+        out[c] = from_f<E>(t);
+    }
+}

@@ -115,3 +115,51 @@ def value_rescale_inv(x: torch.Tensor, eps: float = 1e-3) -> torch.Tensor:
     return torch.sign(x) * (
         ((torch.sqrt(1.0 + 4.0 * eps * (torch.abs(x) + 1.0 + eps)) - 1.0) / (2.0 * eps)) ** 2 - 1.0
     )
+
+
+# ------------------------------------------------------------- layer norm (K9)
+def layer_norm_ref(x, weight, bias=None, eps: float = 1e-5, residual=None):
+    """Layer norm of the last axis of x (+ residual), in 32 bits at least and
+    rounded once. Returns y, or (y, x + residual). Differentiable."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    s = x.to(wide) if residual is None else x.to(wide) + residual.to(wide)
+    var, mean = torch.var_mean(s, dim=-1, unbiased=False, keepdim=True)
+    y = (s - mean) * torch.rsqrt(var + eps) * weight.to(wide)
+    if bias is not None:
+        y = y + bias.to(wide)
+    y = y.to(x.dtype)
+    return y if residual is None else (y, s.to(x.dtype))
+
+
+# ------------------------------------------------ gated linear recurrence (K10)
+def gated_recurrence_ref(gates, h0=None, lengths=None):
+    """h_t = sigma(f) h_{t-1} + sigma(-f) v, y_t = h_t silu(o) over gates
+    [T, B, 3H] = (f, v, o). Steps at or past lengths[b] hold the state, with
+    y = 0. Returns (y [T,B,H], hT [B,H] in 32 bits at least). Differentiable."""
+    wide = torch.promote_types(gates.dtype, torch.float32)
+    T, B, H3 = gates.shape
+    f, v, o = gates.to(wide).split(H3 // 3, dim=-1)
+    h = gates.new_zeros(B, H3 // 3, dtype=wide) if h0 is None else h0.to(wide)
+    ys = []
+    for t in range(T):
+        new = torch.sigmoid(f[t]) * h + torch.sigmoid(-f[t]) * v[t]
+        y = new * o[t] * torch.sigmoid(o[t])
+        if lengths is not None:
+            real = (lengths > t).unsqueeze(1)
+            new, y = torch.where(real, new, h), torch.where(real, y, torch.zeros_like(y))
+        h = new
+        ys.append(y)
+    y = torch.stack(ys) if T else f
+    return y.to(gates.dtype), (h.clone() if T == 0 else h)
+
+
+# ------------------------------------------------------ gated linear unit (K11)
+def gated_linear_ref(x, weight, bias=None):
+    """silu(x Wg^T + bg) * (x Wv^T + bv) with weight [2F, K] = (Wg, Wv), in 32
+    bits at least and rounded once. Differentiable."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    p = x.to(wide) @ weight.to(wide).t()
+    if bias is not None:
+        p = p + bias.to(wide)
+    g, u = p.chunk(2, dim=-1)
+    return (g * torch.sigmoid(g) * u).to(x.dtype)

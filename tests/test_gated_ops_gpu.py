@@ -1,0 +1,405 @@
+"""Layer norm, gated recurrence and gated linear unit kernels against their
+definitions in 64 bits, at the sizes and masks where they can go wrong."""
+
+import pytest
+import torch
+
+from gated_oracles import check, linear_oracle, norm_oracle, recurrence_oracle
+from pytorch_r2d2_dpg_amd.ops.gated_linear import gated_linear
+from pytorch_r2d2_dpg_amd.ops.gated_recurrence import gated_recurrence
+from pytorch_r2d2_dpg_amd.ops.layer_norm import layer_norm
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def rand(*shape, seed=0, dtype=FP32, scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed + 1000 * len(shape))
+    return (torch.randn(*shape, generator=g) * scale + shift).to(dtype).cuda()
+
+
+def leaves(*tensors):
+    for t in tensors:
+        if t is not None:
+            t.requires_grad_(True)
+    return [t for t in tensors if t is not None]
+
+
+def check_all(got, want):
+    assert len(got) == len(want)
+    for i, (g, w) in enumerate(zip(got, want)):
+        check(f"output {i}", g, w)
+
+
+# ------------------------------------------------------------------ layer norm
+def run_norm(rows, dim, dtype, residual, bias=True, seed=0, scale=1.0, shift=0.2):
+    x = rand(rows, dim, seed=seed, dtype=dtype, scale=scale, shift=shift)
+    w = rand(dim, seed=seed + 1, dtype=dtype, scale=0.1, shift=1.0)
+    b = rand(dim, seed=seed + 2, dtype=dtype) if bias else None
+    r = rand(rows, dim, seed=seed + 3, dtype=dtype) if residual else None
+    dy, ds = rand(rows, dim, seed=seed + 4, dtype=dtype), rand(rows, dim, seed=seed + 5, dtype=dtype)
+    ins = leaves(x, w, b, r)
+    out = layer_norm(x, w, b, residual=r)
+    outs, seeds = (list(out), [dy, ds]) if residual else ([out], [dy])
+    grads = list(torch.autograd.grad(outs, ins, seeds))
+    if residual:
+        assert torch.equal(grads[0], grads.pop())  # x and the residual share one gradient
+    check_all(outs + grads, norm_oracle(x, w, b, r, dy, ds if residual else None))
+    with torch.no_grad():  # the same values without gradients
+        again = layer_norm(x, w, b, residual=r)
+    for a, o in zip(again if residual else [again], outs):
+        assert torch.equal(a, o)
+
+
+# each count of threads and runs a row, both sides of every border, and past registers
+@pytest.mark.parametrize("dim", [1, 7, 64, 512, 513, 771, 1025, 2048, 2049, 4100, 8192, 8200, 33000])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_dims(dim, dtype, residual):
+    run_norm(5, dim, dtype, residual, seed=dim)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 3, 4, 2049, 5000])
+@pytest.mark.parametrize("dim", [40, 600])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_norm_rows(rows, dim, dtype):
+    run_norm(rows, dim, dtype, True, bias=rows != 3, seed=rows)
+
+
+def test_norm_far_from_zero_and_constant():
+    run_norm(9, 300, FP32, False, scale=0.01, shift=1000.0)  # the variance must not cancel
+    x = torch.full((3, 70), 2.5, device="cuda")
+    y = layer_norm(x, rand(70), rand(70, seed=1))
+    assert torch.equal(y, rand(70, seed=1).expand(3, 70))
+
+
+def test_norm_keeps_rows_apart():
+    x, w = rand(6, 200), rand(200, seed=1)
+    clean = layer_norm(x, w)
+    bad = x.clone()
+    bad[1, 3], bad[4, 7] = float("nan"), float("inf")
+    y = layer_norm(bad, w)
+    for i in (0, 2, 3, 5):
+        assert torch.equal(y[i], clean[i])
+    assert y[1].isnan().all() and y[4].isnan().any()
+
+
+def test_norm_strides_and_shapes():
+    wide = rand(4, 6, 90, dtype=BF16)
+    x, w = wide[:, ::2, 5:55], rand(100, seed=1, dtype=BF16)[::2]
+    assert torch.equal(layer_norm(x, w), layer_norm(x.contiguous(), w.contiguous()))
+    x0 = wide.view(-1)[1:1 + 23 * 50].view(23, 50)  # rows that start on odd elements
+    dy = rand(23, 50, seed=2, dtype=BF16)
+    ins = leaves(x0.detach(), w.contiguous())
+    y = layer_norm(*ins)
+    check_all([y] + list(torch.autograd.grad([y], ins, [dy])), norm_oracle(*ins, None, None, dy, None))
+
+
+def test_norm_partial_gradients():
+    x, w, r = rand(7, 33), rand(33, seed=1), rand(7, 33, seed=2)
+    ins = leaves(x, w, r)
+    _, s = layer_norm(x, w, residual=r)
+    g = rand(7, 33, seed=3)
+    gx, gw, gr = torch.autograd.grad([s], ins, [g])  # through the sum alone
+    assert torch.equal(gx, g) and torch.equal(gr, g) and not gw.any()
+    y, _ = layer_norm(x, w, residual=r)
+    check_all([torch.autograd.grad([y], [x], [g])[0]],
+              [norm_oracle(x, w, None, r, g, torch.zeros_like(g))[2]])
+
+
+# ------------------------------------------------------------ gated recurrence
+def run_recurrence(T, B, H, dtype, lengths=None, state=True, seed=0):
+    gates = rand(T, B, 3 * H, seed=seed, dtype=dtype)
+    gates[:, :, :H] *= 1.5
+    gates[:, :, :H] += 2
+    h0 = rand(B, H, seed=seed + 1) if state else None
+    dy, dh = rand(T, B, H, seed=seed + 2, dtype=dtype), rand(B, H, seed=seed + 3)
+    if lengths is not None:
+        lengths = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    ins = leaves(gates, h0)
+    outs = list(gated_recurrence(gates, h0, lengths))
+    got = outs + list(torch.autograd.grad(outs, ins, [dy, dh]))
+    want = recurrence_oracle(gates, h0, lengths, dy, dh)
+    check_all(got, want if state else want[:3])
+    with torch.no_grad():
+        for a, o in zip(gated_recurrence(gates, h0, lengths), outs):
+            assert torch.equal(a, o)
+    return got
+
+
+# one step, borders of a wave's chunk, of a block's waves, several passes, segments
+@pytest.mark.parametrize("T", [0, 1, 2, 15, 16, 17, 40, 128, 129, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_recurrence_steps(T, dtype):
+    run_recurrence(T, 3, 70, dtype, seed=T)
+
+
+@pytest.mark.parametrize("B, H", [(1, 1), (1, 2), (5, 3), (33, 64), (2, 129), (7, 200), (0, 8)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_recurrence_channels(B, H, dtype):
+    run_recurrence(37, B, H, dtype, state=H != 64, seed=B + H)
+
+
+@pytest.mark.parametrize("T, B, H", [(3000, 1, 64), (2049, 2, 65), (5000, 3, 8)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_recurrence_long(T, B, H, dtype):
+    run_recurrence(T, B, H, dtype, lengths=[T - 1000, T + 5, 17][:B] if B > 1 else None, seed=T)
+
+
+@pytest.mark.parametrize("T", [1, 16, 75, 400])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_recurrence_lengths(T, dtype):
+    run_recurrence(T, 6, 33, dtype, lengths=[0, 1, T, T + 9, -3, T // 2], seed=T)
+
+
+def test_recurrence_pads_have_no_effect():
+    T, B, H = 50, 4, 48
+    lengths = torch.tensor([0, 13, 32, 50], dtype=torch.int32, device="cuda")
+    got = []
+    for fill in (0.0, float("nan"), float("inf"), torch.finfo(FP32).min):
+        gates, h0 = rand(T, B, 3 * H), rand(B, H, seed=1)
+        dy, dh = rand(T, B, H, seed=2), rand(B, H, seed=3)
+        for b, n in enumerate(lengths.tolist()):
+            gates[n:, b], dy[n:, b] = fill, fill
+        ins = leaves(gates, h0)
+        outs = list(gated_recurrence(gates, h0, lengths))
+        got.append(outs + list(torch.autograd.grad(outs, ins, [dy, dh])))
+    y, hT, dg, dh0 = got[0]
+    for b, n in enumerate(lengths.tolist()):
+        assert not y[n:, b].any() and not dg[n:, b].any()
+    assert torch.equal(hT[0], rand(B, H, seed=1)[0]) and torch.equal(dh0[0], rand(B, H, seed=3)[0])
+    for other in got[1:]:
+        for a, o in zip(other, got[0]):
+            assert torch.equal(a, o)
+
+
+def test_recurrence_saturated_gates():
+    T, B, H = 20, 2, 32
+    for f in (float("inf"), 200.0, -200.0, float("-inf")):
+        gates, h0 = rand(T, B, 3 * H), rand(B, H, seed=1)
+        gates[:, :, :H] = f
+        ins = leaves(gates, h0)
+        y, hT = gated_recurrence(gates, h0)
+        assert torch.equal(hT, h0 if f > 0 else gates[-1, :, H:2 * H])
+        for g in torch.autograd.grad([y, hT], ins, [torch.ones_like(y), torch.ones_like(hT)]):
+            assert g.isfinite().all()
+
+
+def test_recurrence_in_pieces():
+    """One step a call, as a serving loop makes them, ends where one call does."""
+    T, B, H = 40, 5, 72
+    gates, h0 = rand(T, B, 3 * H, dtype=BF16), rand(B, H, seed=1)
+    want = recurrence_oracle(gates, h0, None, None, None)
+    with torch.no_grad():
+        h, ys = h0, []
+        for t in range(T):
+            y, h = gated_recurrence(gates[t:t + 1], h)
+            ys.append(y)
+    check_all([torch.cat(ys), h], want[:2])
+
+
+def test_recurrence_strides_and_partial_gradients():
+    T, B, H = 30, 4, 20
+    gates = rand(B, T, 3 * H).transpose(0, 1)
+    dy = rand(B, T, H, seed=1).transpose(0, 1)
+    ins = leaves(gates.detach())
+    y, hT = gated_recurrence(*ins)
+    want = recurrence_oracle(gates, None, None, dy, None)
+    check_all([y, hT, torch.autograd.grad([y], ins, [dy])[0]], want[:3])
+    dh = rand(B, H, seed=2)
+    y, hT = gated_recurrence(*ins)
+    check_all([torch.autograd.grad([hT], ins, [dh])[0]],
+              [recurrence_oracle(gates, None, None, None, dh)[2]])
+
+
+def test_recurrence_offsets_past_32_bits():
+    T, B, H = 2816, 512, 512  # 2.2e9 gate values
+    gates = torch.randn(T, 1, 3 * H, device="cuda", dtype=BF16).repeat(1, B, 1)
+    gates[:, -1] = rand(T, 3 * H, dtype=BF16)
+    ins = leaves(gates)
+    dy = torch.ones(T, B, H, device="cuda", dtype=BF16)
+    y, hT = gated_recurrence(gates)
+    dg = torch.autograd.grad([y], ins, [dy])[0]
+    want = recurrence_oracle(gates[:, -1:], None, None, dy[:, -1:], None)
+    check_all([y[:, -1:], hT[-1:], dg[:, -1:]], want[:3])
+    assert torch.equal(y[:, 0], y[:, -2]) and torch.equal(dg[:, 0], dg[:, -2])
+
+
+# ----------------------------------------------------------- gated linear unit
+def run_linear(M, K, F, dtype, bias=True, seed=0, shape=None):
+    x = rand(M, K, seed=seed, dtype=dtype).reshape(shape or (M, K))
+    w = rand(2 * F, K, seed=seed + 1, dtype=dtype, scale=max(K, 1) ** -0.5)
+    b = rand(2 * F, seed=seed + 2, dtype=dtype, scale=0.3) if bias else None
+    dy = rand(M, F, seed=seed + 3, dtype=dtype).reshape(*x.shape[:-1], F)
+    ins = leaves(x, w, b)
+    y = gated_linear(x, w, b)
+    got = [y] + list(torch.autograd.grad([y], ins, [dy]))
+    want = linear_oracle(x, w, b, dy)
+    check_all(got, want)
+    for g, (exact, _) in zip(got, want):
+        # Errors of independent signs: the result's own rounding, and dp's, whose
+        # share of a sum is half of its norm at most.
+        if M * F * K and exact.numel() > 64:
+            off = (g.detach().double().cpu() - exact).norm() / exact.norm()
+            assert off < 2 * torch.finfo(dtype).eps / 2 + 64 * 2.0 ** -24, float(off)
+    with torch.no_grad():
+        assert torch.equal(gated_linear(x, w, b), y)
+    return got
+
+
+@pytest.mark.parametrize("M", [0, 1, 2, 15, 17, 64, 65, 129, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_linear_rows(M, dtype):
+    run_linear(M, 72, 80, dtype, seed=M)
+
+
+@pytest.mark.parametrize("K", [1, 7, 8, 31, 64, 203, 520])
+@pytest.mark.parametrize("F", [1, 16, 33, 129, 264])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_linear_widths(K, F, dtype):
+    run_linear(70, K, F, dtype, bias=F != 16, seed=K + F)
+
+
+@pytest.mark.parametrize("M, K, F", [(1500, 512, 1024), (5000, 96, 64), (33, 2048, 512)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_linear_larger(M, K, F, dtype):
+    run_linear(M, K, F, dtype, seed=M)
+
+
+def test_linear_shapes_strides_and_partial_gradients():
+    run_linear(24, 40, 32, BF16, shape=(2, 3, 4, 40))
+    x, w = rand(60, 9, 50, dtype=BF16)[::3, 2, 3:43], rand(40, 48, seed=1, dtype=BF16).t()
+    b = rand(48, seed=2, dtype=BF16)
+    assert torch.equal(gated_linear(x, w, b), gated_linear(x.contiguous(), w.contiguous(), b))
+    dy = rand(20, 24, seed=3, dtype=BF16)
+    want = linear_oracle(x, w, b, dy)
+    for pick in ([0], [1], [2], [0, 2]):
+        ins = [x.detach().contiguous(), w.detach().contiguous(), b.detach()]
+        for i in pick:
+            ins[i].requires_grad_(True)
+        y = gated_linear(*ins)
+        check_all(torch.autograd.grad([y], [ins[i] for i in pick], [dy]), [want[1 + i] for i in pick])
+    # rows that start on odd elements
+    flat = rand(21 * 40 + 1, dtype=BF16)
+    x = flat[1:].view(21, 40)
+    assert torch.equal(gated_linear(x, w), gated_linear(x.clone(), w))
+
+
+def test_linear_keeps_rows_apart():
+    x, w = rand(70, 96, dtype=BF16), rand(64, 96, seed=1, dtype=BF16)
+    clean = gated_linear(x, w)
+    bad = x.clone()
+    bad[5, 3], bad[69, 0] = float("nan"), float("inf")
+    y = gated_linear(bad, w)
+    same = [i for i in range(70) if i not in (5, 69)]
+    assert torch.equal(y[same], clean[same]) and y[5].isnan().all()
+
+
+# ----------------------------------------------------- refusals, streams, graphs
+def test_gpu_refusals():
+    x, w = rand(3, 8), rand(8, seed=1)
+    with pytest.raises(RuntimeError):
+        layer_norm(x.half(), w.half())
+    with pytest.raises(RuntimeError):
+        layer_norm(x, w.cpu())
+    with pytest.raises(RuntimeError):
+        gated_recurrence(rand(2, 3, 6).half())
+    with pytest.raises(RuntimeError):
+        gated_recurrence(rand(2, 3, 6), None, torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(RuntimeError):
+        gated_linear(x, rand(4, 8).cpu())
+    y = layer_norm(x.requires_grad_(True), w)
+    g = torch.autograd.grad(y.sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+def block(p, gates_of):
+    """The three as a residual block uses them; returns outputs and gradients."""
+    n = layer_norm(p["x"], p["w1"], p["b1"])
+    y, hT = gated_recurrence(gates_of(n), p["h0"])
+    n2, s = layer_norm(y, p["w2"], p["b2"], residual=p["x"])
+    out = gated_linear(n2, p["wl"], p["bl"]) + s
+    ins = [p[k] for k in ("x", "w1", "b1", "wg", "h0", "w2", "b2", "wl", "bl")]
+    return [out, hT] + list(torch.autograd.grad([out, hT], ins, [p["dy"], p["dh"]]))
+
+
+def block_inputs(dtype, T=33, B=5, H=64, seed=0):
+    p = {"x": rand(T, B, H, seed=seed, dtype=dtype), "wg": rand(3 * H, H, seed=seed + 1, dtype=dtype, scale=H ** -0.5),
+         "h0": rand(B, H, seed=seed + 2), "wl": rand(2 * H, H, seed=seed + 3, dtype=dtype, scale=H ** -0.5),
+         "bl": rand(2 * H, seed=seed + 4, dtype=dtype)}
+    for i, k in enumerate(("w1", "b1", "w2", "b2")):
+        p[k] = rand(H, seed=seed + 5 + i, dtype=dtype, scale=0.1, shift=float(k[0] == "w"))
+    leaves(*p.values())
+    p["dy"], p["dh"] = rand(T, B, H, seed=seed + 9, dtype=dtype), rand(B, H, seed=seed + 10)
+    return p
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_together_against_64_bits(dtype):
+    p = block_inputs(dtype)
+    got = block(p, lambda n: n @ p["wg"].t())
+    q = {k: v.detach().double().cpu() for k, v in p.items()}
+    leaves(*[q[k] for k in q if k not in ("dy", "dh")])
+    want = block(q, lambda n: n @ q["wg"].t())
+    # five roundings to the type lie on the longest path, each of half a step, and
+    # the norms and gates carry them on no larger than the values' own norm
+    bound = 5 * torch.finfo(dtype).eps / 2 * 2 + 256 * 2.0 ** -24
+    for i, (g, w) in enumerate(zip(got, want)):
+        off = (g.detach().double().cpu() - w).norm() / w.norm()
+        assert off < bound, (i, float(off))
+
+
+def test_streams():
+    p, q = block_inputs(BF16), block_inputs(BF16, seed=50)
+    want = [block(s, lambda n, s=s: n @ s["wg"].t()) for s in (p, q)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for _ in range(3):
+        for i, s in enumerate((p, q)):
+            with torch.cuda.stream(streams[i]):
+                got[i] = block(s, lambda n, s=s: n @ s["wg"].t())
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            assert torch.equal(a, b)
+
+
+def test_two_graphs_replayed():
+    cases = [block_inputs(BF16), block_inputs(BF16, T=300, B=2, seed=50)]
+    graphs, outs = [], []
+    for p in cases:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block(p, lambda n: n @ p["wg"].t())
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(block(p, lambda n: n @ p["wg"].t()))
+        graphs.append(graph)
+    for turn in range(3):
+        for i, p in enumerate(cases):
+            with torch.no_grad():
+                p["x"].copy_(rand(*p["x"].shape, seed=90 + turn, dtype=BF16))
+                p["dy"].copy_(rand(*p["dy"].shape, seed=70 + turn, dtype=BF16))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for p, out in zip(cases, outs):
+            for a, b in zip(out, block(p, lambda n: n @ p["wg"].t())):
+                assert torch.equal(a, b)
+
+
+def test_capture_over_a_live_eager_graph_is_refused():
+    x, w = rand(4, 16), rand(16, seed=1).requires_grad_(True)
+    alive = layer_norm(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            layer_norm(x, w)
+    del alive
+    y = layer_norm(x, w)
+    assert torch.equal(torch.autograd.grad([y], [w], [torch.ones_like(y)])[0].isfinite(),
+                       torch.ones(16, dtype=torch.bool, device="cuda"))
