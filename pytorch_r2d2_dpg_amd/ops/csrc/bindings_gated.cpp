@@ -21,8 +21,8 @@ extern "C" int launch_norm_fwd(int, const void*, const void*, const void*, const
                                void*, int64_t, int, float, hipStream_t);
 extern "C" int norm_bwd_parts(int, int64_t, int);
 extern "C" int64_t norm_bwd_stats(int, int64_t, int);
-extern "C" int launch_norm_bwd(int, const void*, const void*, const void*, const void*, void*,
-                               float*, float*, void*, int64_t, int, int, float, hipStream_t);
+extern "C" int launch_norm_bwd(int, const void*, const void*, const void*, const void*,
+                               const void*, void*, float*, float*, void*, int64_t, int, int, float, hipStream_t);
 extern "C" int recurrence_chunk();
 extern "C" int64_t recurrence_maps(int, int, int);
 extern "C" int launch_recurrence_fwd(int, const void*, const float*, const int*, void*, float*,
@@ -32,8 +32,8 @@ extern "C" int launch_recurrence_bwd(int, const void*, const float*, const int*,
                                      hipStream_t);
 extern "C" int launch_gated_linear_fwd(int, const void*, const void*, const void*, void*, int,
                                        int, int, hipStream_t);
-extern "C" int gated_linear_bias_parts(int);
-extern "C" int gated_linear_splits(int, int, int);
+extern "C" int gated_linear_bias_parts(int, int, int);
+extern "C" int gated_linear_splits(int, int, int, int);
 extern "C" int launch_gated_linear_bwd(int, const void*, const void*, const void*, const void*,
                                        void*, void*, void*, void*, float*, float*, int, int, int,
                                        int, hipStream_t);
@@ -87,24 +87,25 @@ std::tuple<Tensor, Tensor> layer_norm_fwd(Tensor x, Tensor weight, OptTensor bia
     return {y, s};
 }
 
-std::tuple<Tensor, Tensor> layer_norm_bwd(Tensor s, Tensor weight, Tensor dy, OptTensor ds,
-                                          double eps) {
-    check_first(s, "s");
-    TORCH_CHECK(s.dim() >= 1 && s.size(-1) > 0, "s must have a last axis to normalise");
-    const c10::DeviceGuard guard(s.device());
-    const int64_t dim = s.size(-1), rows = s.numel() / dim;
-    TORCH_CHECK(dim <= MOST && rows <= MOST, "s is too large");
-    check(weight, "weight", s, s.scalar_type(), {dim});
-    check(dy, "dy", s, s.scalar_type(), s.sizes());
-    if (ds) check(*ds, "ds", s, s.scalar_type(), s.sizes());
-    const int parts = norm_bwd_parts(is_bf16(s), rows, (int)dim);
-    const auto f32 = s.options().dtype(torch::kFloat32);
-    auto dx = torch::empty_like(s);
-    auto dwb = torch::empty({2, dim}, s.options());
+std::tuple<Tensor, Tensor> layer_norm_bwd(Tensor x, OptTensor residual, Tensor weight, Tensor dy,
+                                          OptTensor ds, double eps) {
+    check_first(x, "x");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have a last axis to normalise");
+    const c10::DeviceGuard guard(x.device());
+    const int64_t dim = x.size(-1), rows = x.numel() / dim;
+    TORCH_CHECK(dim <= MOST && rows <= MOST, "x is too large");
+    check(weight, "weight", x, x.scalar_type(), {dim});
+    check(dy, "dy", x, x.scalar_type(), x.sizes());
+    if (residual) check(*residual, "residual", x, x.scalar_type(), x.sizes());
+    if (ds) check(*ds, "ds", x, x.scalar_type(), x.sizes());
+    const int parts = norm_bwd_parts(is_bf16(x), rows, (int)dim);
+    const auto f32 = x.options().dtype(torch::kFloat32);
+    auto dx = torch::empty_like(x);
+    auto dwb = torch::empty({2, dim}, x.options());
     auto part = torch::empty({parts, 2 * dim}, f32);
-    auto stats = torch::empty({norm_bwd_stats(is_bf16(s), rows, (int)dim)}, f32);
-    const int rc = launch_norm_bwd(is_bf16(s), s.data_ptr(), weight.data_ptr(), dy.data_ptr(),
-                                   ptr(ds), dx.data_ptr(), part.data_ptr<float>(),
+    auto stats = torch::empty({norm_bwd_stats(is_bf16(x), rows, (int)dim)}, f32);
+    const int rc = launch_norm_bwd(is_bf16(x), x.data_ptr(), ptr(residual), weight.data_ptr(),
+                                   dy.data_ptr(), ptr(ds), dx.data_ptr(), part.data_ptr<float>(),
                                    stats.data_ptr<float>(), dwb.data_ptr(), rows, (int)dim, parts,
                                    (float)eps, stream());
     TORCH_CHECK(rc == 0, "layer norm backward launch failed");
@@ -173,8 +174,10 @@ LinearSizes check_linear(const Tensor& x, const Tensor& weight, const OptTensor&
     if (bias) check(*bias, "bias", x, x.scalar_type(), {2 * F});
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
-    // blocks of rows lie on a grid axis of 65535
-    TORCH_CHECK(M <= 64 * 65535LL && K <= MOST && F <= 32 * 65535LL, "x or weight is too large");
+    // tiles of 128 by 64 at the least lie on one grid axis
+    TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST && (M / 128 + 1) * (F / 64 + 1) <= MOST &&
+                    (M / 128 + 1) * (K / 64 + 1) <= MOST && (F / 64 + 1) * (K / 64 + 1) <= MOST,
+                "x or weight is too large");
     return {M, K, F};
 }
 
@@ -201,15 +204,15 @@ std::tuple<Tensor, Tensor, Tensor> gated_linear_bwd(Tensor x, Tensor weight, Opt
     const auto f32 = x.options().dtype(torch::kFloat32);
     auto dp = torch::empty({n.M, 2 * n.F}, x.options());
     Tensor dx, dw, db, part_db, part_dw;
-    const int splits = gated_linear_splits((int)n.M, (int)n.K, (int)n.F);
+    const int splits = gated_linear_splits(is_bf16(x), (int)n.M, (int)n.K, (int)n.F);
     if (need_x) dx = torch::empty_like(x);
     if (need_w) {
         dw = torch::empty_like(weight);
-        part_dw = torch::empty({splits, 2 * n.F, n.K}, f32);
+        part_dw = torch::empty({splits > 1 ? splits : 0, 2 * n.F, n.K}, f32);
     }
     if (need_b) {
         db = torch::empty({2 * n.F}, x.options());
-        part_db = torch::empty({gated_linear_bias_parts((int)n.M), 2 * n.F}, f32);
+        part_db = torch::empty({gated_linear_bias_parts(is_bf16(x), (int)n.M, (int)n.F), 2 * n.F}, f32);
     }
     const int rc = launch_gated_linear_bwd(
         is_bf16(x), x.data_ptr(), weight.data_ptr(), ptr(bias), dy.data_ptr(), dp.data_ptr(),

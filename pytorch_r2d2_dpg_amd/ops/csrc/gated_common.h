@@ -77,7 +77,7 @@ DEV_INLINE float wave_sum(float v) {
 // a reduction over rows, in place of atomics whose order would change results.
 // 16 waves share 64 columns, wave w the rows w, w+16, ...
 template <typename E>
-__global__ void __launch_bounds__(1024)
+static __global__ void __launch_bounds__(1024)
 column_sum_kernel(const float* __restrict__ part, E* __restrict__ out,
                   int rows, int cols) {
     __shared__ float sums[16][64];

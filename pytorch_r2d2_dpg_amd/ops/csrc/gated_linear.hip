@@ -10,7 +10,8 @@
 // indexes, so each lane ends with g and u of the same elements, and the
 // activation, the product and (backward) dp are written from the accumulators.
 // The backward pass computes g and u again in place of keeping them: nothing
-// but the inputs lives between the passes, and g and u are never rounded.
+// but the inputs lives between the passes, and g and u are never rounded. dp is
+// rounded to the type, as the matrix instructions of the next products take it.
 
 #include "gated_common.h"
 
@@ -18,138 +19,343 @@ namespace {
 
 using f4 = __attribute__((ext_vector_type(4))) float;
 using bf8 = __attribute__((ext_vector_type(8))) __bf16;
+using s4 = __attribute__((ext_vector_type(4))) short;
+using u4 = __attribute__((ext_vector_type(4))) unsigned int;
+#define LDS_PTR(T) __attribute__((address_space(3))) T*
 
-constexpr int TILE = 64, DEPTH = 32;
+// Tiles are handled in pieces of 16 bytes: PIECE elements.
+template <typename E> constexpr int PIECE = 16 / (int)sizeof(E);
+// k of one tile: 128 bytes of it.
+template <typename E> constexpr int DEPTH = 128 / (int)sizeof(E);
 
-// What the matrix instruction takes of a lane: KL values of consecutive k, of
-// the row (or column) lane % 16, at k = (lane / 16) * KL.
-template <typename E> struct Mfma;
-template <> struct Mfma<bf16> {
-    static constexpr int STEP = 32, KL = 8;
-    static DEV_INLINE f4 mul(const bf16* a, const bf16* b, f4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf8*>(a),
-                                                       *reinterpret_cast<const bf8*>(b), c, 0, 0, 0);
+// Reads as zeros wherever a piece lies past the operand's end.
+__device__ const u4 nothing = {0, 0, 0, 0};
+
+// A lane's piece holds k = 4 groups of PIECE, group lane / 16, of one row (or
+// column) lane % 16. bf16 takes the piece in one instruction; fp32 in four of
+// k = 4, the s-th taking element s of every group.
+DEV_INLINE f4 mul(bf16, u4 a, u4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a),
+                                                   __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+DEV_INLINE f4 mul(float, u4 a, u4 b, f4 c) {
+    const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s], y[s], c, 0, 0, 0);
+    return c;
+}
+
+// How an operand lies in memory: k together (rows of it are the result's rows or
+// columns), or the result's index together (rows of it are k).
+enum class Lie { K, INDEX };
+
+// One operand's tile of SPAN indexes by DEPTH k, in LDS as the operand lies in
+// memory, its pieces permuted so that the lanes that read together meet
+// different banks: by the row's low bits where k lies together, by pairs of
+// pieces and k's low two bits for the transposing reads.
+template <typename E, Lie LIE, int SPAN, int THREADS, bool DIRECT>
+struct Operand {
+    static constexpr int P = PIECE<E>, PIECES = SPAN * 8, ROUNDS = PIECES / THREADS;
+    static constexpr int ROW = LIE == Lie::K ? 8 : SPAN / P;  // pieces of a row in LDS
+    static_assert(PIECES % THREADS == 0, "every thread stages as many pieces");
+
+    const E* at[ROUNDS];  // this thread's pieces of the tile at k = 0
+    int have[ROUNDS];     // elements of it along the index (INDEX), 0 or less: none
+    u4 held[DIRECT ? 1 : ROUNDS];
+
+    static DEV_INLINE int swizzle(int row, int piece) {
+        return LIE == Lie::K ? piece ^ (row & 7)
+                             : sizeof(E) == 2 ? piece ^ ((row & 3) << 1) : piece;
     }
-};
-template <> struct Mfma<float> {
-    static constexpr int STEP = 4, KL = 1;
-    static DEV_INLINE f4 mul(const float* a, const float* b, f4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x4f32(*a, *b, c, 0, 0, 0);
+
+    // `index(i)`: the operand's index for the tile's i-th, inside of it always
+    // (K) or the first of a run (INDEX); `count`: how many indexes there are.
+    template <typename F>
+    DEV_INLINE void start(const E* base, int64_t pitch, int count, F&& index) {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const int slot = r * THREADS + threadIdx.x, row = slot / ROW;
+            const int piece = swizzle(row, slot % ROW);
+            if constexpr (LIE == Lie::K) {
+                at[r] = base + index(row) * pitch + piece * P;
+                have[r] = piece * P;  // its k
+            } else {
+                const int64_t i = index(piece * P);
+                at[r] = base + row * pitch + i;
+                have[r] = i < count ? (int)(count - i < P ? count - i : P) : 0;
+            }
+        }
+    }
+
+    // Elements of a piece that exist in the tile at k0.
+    DEV_INLINE int left(int r, int k0, int k_hi) const {
+        if constexpr (LIE == Lie::K) return k_hi - k0 - have[r];
+        else return k0 + (r * THREADS + (int)threadIdx.x) / ROW < k_hi ? have[r] : 0;
+    }
+
+    DEV_INLINE void fetch(u4* tile, int64_t pitch, int k0, int k_hi) {
+        const int64_t step = LIE == Lie::K ? k0 : (int64_t)k0 * pitch;
+        const bool whole = k0 + DEPTH<E> <= k_hi;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const E* p = at[r] + step;
+            if constexpr (DIRECT) {
+                // aligned pitches: a piece exists whole or not at all
+                if (LIE == Lie::INDEX || !whole)
+                    if (left(r, k0, k_hi) <= 0) p = reinterpret_cast<const E*>(&nothing);
+                u4* to = tile + r * THREADS + (threadIdx.x & ~63);
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass takes 16 bytes for an error
+                __builtin_amdgcn_global_load_lds(p, (LDS_PTR(void))to, 16, 0, 0);
+#endif
+            } else {
+                E v[P];
+                const int n = LIE == Lie::K && whole ? P : left(r, k0, k_hi);
+                load_run<E, P>(p, n, v);
+                held[r] = __builtin_bit_cast(u4, v);
+            }
+        }
+    }
+
+    DEV_INLINE void settle(u4* tile) const {
+        if constexpr (!DIRECT)
+#pragma unroll
+            for (int r = 0; r < ROUNDS; ++r) tile[r * THREADS + threadIdx.x] = held[r];
+    }
+
+    // The piece of the matrix instructions for the 16 indexes from `first`, at
+    // the tile's k from `k` pieces of four groups on.
+    static DEV_INLINE u4 read(const u4* tile, int first, int k) {
+        const int lane = threadIdx.x & 63, group = lane >> 4;
+        if constexpr (LIE == Lie::K) {
+            const int row = first + (lane & 15);
+            return tile[row * 8 + swizzle(row, k * 4 + group)];
+        } else if constexpr (sizeof(E) == 2) {
+            // 16 lanes read 4 k by 16 indexes, 8 bytes each, and get back the 4 k
+            // of one index each
+            u4 out;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = k * 32 + group * 8 + h * 4 + ((lane & 15) >> 2);
+                const int i = first + (lane & 3) * 4;
+                const char* p = (const char*)(tile + row * ROW + swizzle(row, i / P)) + (i % P) * 2;
+                const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s4))p);
+                out[2 * h] = __builtin_bit_cast(u4, (__attribute__((ext_vector_type(8))) short){
+                    v[0], v[1], v[2], v[3], 0, 0, 0, 0})[0];
+                out[2 * h + 1] = __builtin_bit_cast(u4, (__attribute__((ext_vector_type(8))) short){
+                    v[0], v[1], v[2], v[3], 0, 0, 0, 0})[1];
+            }
+            return out;
+        } else {
+            const float* f = reinterpret_cast<const float*>(tile);
+            u4 out;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                out[s] = __builtin_bit_cast(unsigned,
+                    f[(k * 16 + group * 4 + s) * SPAN + first + (lane & 15)]);
+            return out;
+        }
     }
 };
 
 enum class End { GATED, GATED_GRAD, PLAIN, PART };
 
-// C(m, n) = sum over k of A(m, k) B(n, k); A and B have strides for both axes.
+// C(m, n) = sum over k of A(m, k) B(n, k).
 template <typename E>
 struct Args {
     const E *a, *b;
-    int64_t am, ak, bn, bk;
-    int M, N, K;       // GATED*: N is F
-    const E* bias;     // [2F] or null
-    const E* dy;       // [M, F]
-    E* out;            // GATED: y [M, F]; GATED_GRAD: dp [M, 2F]; PLAIN: [M, N]
-    float* part;       // GATED_GRAD: [blocks of rows, 2F] or null; PART: [splits, M, N]
-    int per_split;     // k of one split
+    int64_t pitch_a, pitch_b;
+    int M, N, K;        // GATED*: N is F
+    const E* bias;      // [2F] or null
+    const E* dy;        // [M, F]
+    E* out;             // GATED: y [M, F]; GATED_GRAD: dp [M, 2F]; PLAIN: [M, N]
+    float* part;        // GATED_GRAD: [tiles of M, 2F] or null; PART: [splits, M, N]
+    int tiles_m, tiles_n, per_split;
 };
 
-template <typename E, End END>
-__global__ void __launch_bounds__(256)
+// Blocks go round the 8 XCDs by their index. Each XCD, which has an L2 of its
+// own, gets a run of tiles, in patches of 8 rows of tiles: those in flight
+// share their operands.
+DEV_INLINE void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int total = tiles_m * tiles_n, q = total / 8, r = total % 8;
+    const int xcd = id % 8, i = id / 8;
+    const int t = xcd * q + (xcd < r ? xcd : r) + i;
+    const int patch = t / (8 * tiles_n), first = patch * 8;
+    const int rows = tiles_m - first < 8 ? tiles_m - first : 8;
+    const int in = t - patch * 8 * tiles_n;
+    tm = first + in % rows;
+    tn = in / rows;
+}
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
+    static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+};
+
+template <typename E, typename T, Lie LA, Lie LB, End END, bool DIRECT>
+__global__ void __launch_bounds__(T::THREADS)
 product_kernel(Args<E> p) {
     constexpr bool GATED = END == End::GATED || END == End::GATED_GRAD;
-    constexpr int PAD = 16 / sizeof(E), STEP = Mfma<E>::STEP, KL = Mfma<E>::KL;
-    constexpr int COLS = GATED ? TILE / 2 : TILE;  // columns of the result a block
-    __shared__ __attribute__((aligned(16))) E as[TILE][DEPTH + PAD], bs[TILE][DEPTH + PAD];
+    constexpr int HALF = T::BN / 2, COLS = GATED ? HALF : T::BN;  // of the result a block
+    constexpr int PIECES = (T::BM + T::BN) * 8, BD = DEPTH<E>;
+    __shared__ u4 lds[2][PIECES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int m0 = blockIdx.y * TILE, n0 = blockIdx.x * COLS;
+    const int wm = wave / T::WN, wn = wave % T::WN;
+    int tm, tn;
+    tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = tm * T::BM, n0 = tn * COLS;
     const int k_lo = blockIdx.z * p.per_split;
     const int k_hi = k_lo + p.per_split < p.K ? k_lo + p.per_split : p.K;
-    // wave (wm, wn): rows wm * 32.., and columns wn * 32.. of the plain forms, or
-    // gate columns wn * 16.. with their value columns of the gated ones
-    const int wm = wave >> 1, wn = wave & 1;
-    f4 acc[2][2] = {};
-    for (int k0 = k_lo; k0 < k_hi; k0 += DEPTH) {
-        __syncthreads();
-        for (int e = threadIdx.x; e < TILE * DEPTH; e += 256) {
-            // neighbours in the axis that lies together in memory
-            const int am = p.ak == 1 ? e / DEPTH : e % TILE, ak = p.ak == 1 ? e % DEPTH : e / TILE;
-            const int m = m0 + am, ka = k0 + ak;
-            as[am][ak] = m < p.M && ka < k_hi ? p.a[m * p.am + ka * p.ak] : from_f<E>(0.0f);
-            const int bn = p.bk == 1 ? e / DEPTH : e % TILE, bk = p.bk == 1 ? e % DEPTH : e / TILE;
-            const int col = n0 + (GATED ? bn % COLS : bn), kb = k0 + bk;
-            const int64_t row = GATED && bn >= COLS ? (int64_t)col + p.N : col;
-            bs[bn][bk] = col < p.N && kb < k_hi ? p.b[row * p.bn + kb * p.bk] : from_f<E>(0.0f);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < DEPTH; k += STEP) {
-            const int at = k + (lane >> 4) * KL;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int r = wm * 32 + i * 16 + (lane & 15);
-                    const int c = (GATED ? j * COLS + wn * 16 : wn * 32 + j * 16) + (lane & 15);
-                    acc[i][j] = Mfma<E>::mul(&as[r][at], &bs[c][at], acc[i][j]);
-                }
-        }
+
+    Operand<E, LA, T::BM, T::THREADS, DIRECT> a;
+    Operand<E, LB, T::BN, T::THREADS, DIRECT> b;
+    a.start(p.a, p.pitch_a, p.M, [&](int i) {
+        const int m = m0 + i;  // rows past the end read the last one: none is stored
+        return (int64_t)(LA == Lie::K && m >= p.M ? p.M - 1 : m);
+    });
+    b.start(p.b, p.pitch_b, p.N, [&](int i) {
+        const int n = n0 + (GATED ? i % HALF : i);
+        const int in = LB == Lie::K && n >= p.N ? p.N - 1 : n;
+        return (int64_t)in + (GATED && i >= HALF ? p.N : 0);
+    });
+
+    f4 acc[T::MI][T::NI] = {};
+    int turn = 0;
+    if (k_lo < k_hi) {
+        a.fetch(lds[0], p.pitch_a, k_lo, k_hi);
+        b.fetch(lds[0] + T::BM * 8, p.pitch_b, k_lo, k_hi);
+        a.settle(lds[0]);
+        b.settle(lds[0] + T::BM * 8);
     }
-    // an accumulator's element q is at row (lane / 16) * 4 + q, column lane % 16
-    if constexpr (GATED) {
-        __shared__ float sums[2][2][COLS];
-        const int col = n0 + wn * 16 + (lane & 15);
-        float sg = 0.0f, su = 0.0f;
-        if (col < p.N) {
-            const float bg = p.bias ? to_f(p.bias[col]) : 0.0f;
-            const float bu = p.bias ? to_f(p.bias[p.N + col]) : 0.0f;
+    for (int k0 = k_lo; k0 < k_hi; k0 += BD) {
+        // this tile has landed, and everyone is done with the other buffer
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        const u4* now = lds[turn];
+        u4* next = lds[turn ^ 1];
+        const bool more = k0 + BD < k_hi;
+        if (more) {
+            a.fetch(next, p.pitch_a, k0 + BD, k_hi);
+            b.fetch(next + T::BM * 8, p.pitch_b, k0 + BD, k_hi);
+        }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int k = 0; k < 2; ++k) {
+            u4 af[T::MI], bf[T::NI];
+#pragma unroll
+            for (int j = 0; j < T::NI; ++j) {
+                // gated: the wave's first half of columns are gates, then their values
+                constexpr int NH = T::NI / 2;
+                const int first = GATED ? (j / NH) * HALF + (wn * NH + j % NH) * 16
+                                        : (wn * T::NI + j) * 16;
+                bf[j] = b.read(now + T::BM * 8, first, k);
+            }
+#pragma unroll
+            for (int i = 0; i < T::MI; ++i) af[i] = a.read(now, (wm * T::MI + i) * 16, k);
+#pragma unroll
+            for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+                for (int j = 0; j < T::NI; ++j) acc[i][j] = mul(E(), bf[j], af[i], acc[i][j]);
+        }
+        if (more) {
+            a.settle(next);
+            b.settle(next + T::BM * 8);
+        }
+        turn ^= 1;
+    }
+
+    // an accumulator's element q: row lane % 16, column (lane / 16) * 4 + q
+    const int row0 = m0 + wm * T::MI * 16 + (lane & 15);
+    if constexpr (GATED) {
+        constexpr int NH = T::NI / 2;
+        float* sums = reinterpret_cast<float*>(lds);  // [WM][2][HALF]
+        if (END == End::GATED_GRAD && p.part) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+            const int in = (wn * NH + j) * 16 + (lane >> 4) * 4, col = n0 + in, have = p.N - col;
+            E bg[4], bu[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) bg[q] = bu[q] = from_f<E>(0.0f);
+            if (p.bias && have > 0) {
+                load_run<E, 4>(p.bias + col, have, bg);
+                load_run<E, 4>(p.bias + p.N + col, have, bu);
+            }
+            float sg[4] = {}, su[4] = {};
+#pragma unroll
+            for (int i = 0; i < T::MI; ++i) {
+                const int row = row0 + i * 16;
+                if (row >= p.M || have <= 0) continue;
+                E out[4], out2[4], d[4];
+                if (END == End::GATED_GRAD) load_run<E, 4>(p.dy + (int64_t)row * p.N + col, have, d);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int row = m0 + wm * 32 + i * 16 + (lane >> 4) * 4 + q;
-                    if (row >= p.M) continue;
-                    const float g = acc[i][0][q] + bg, u = acc[i][1][q] + bu;
+                    const float g = acc[i][j][q] + to_f(bg[q]);
+                    const float u = acc[i][j + NH][q] + to_f(bu[q]);
                     float val, grad;
                     silu_grad(g, val, grad);
                     if (END == End::GATED) {
-                        p.out[(int64_t)row * p.N + col] = from_f<E>(val * u);
+                        out[q] = from_f<E>(val * u);
                     } else {
-                        const float d = to_f(p.dy[(int64_t)row * p.N + col]);
-                        const float dg = d * u * grad, du = d * val;
-                        p.out[(int64_t)row * 2 * p.N + col] = from_f<E>(dg);
-                        p.out[(int64_t)row * 2 * p.N + p.N + col] = from_f<E>(du);
-                        sg += dg;
-                        su += du;
+                        const float dg = to_f(d[q]) * u * grad, du = to_f(d[q]) * val;
+                        out[q] = from_f<E>(dg);
+                        out2[q] = from_f<E>(du);
+                        sg[q] += dg;
+                        su[q] += du;
+                    }
+                }
+                if (END == End::GATED) {
+                    store_run<E, 4>(p.out + (int64_t)row * p.N + col, have, out);
+                } else {
+                    E* to = p.out + (int64_t)row * 2 * p.N + col;
+                    store_run<E, 4>(to, have, out);
+                    store_run<E, 4>(to + p.N, have, out2);
+                }
+            }
+            if (END == End::GATED_GRAD && p.part)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                    for (int s = 1; s < 16; s <<= 1) {
+                        sg[q] += __shfl_xor(sg[q], s, 64);
+                        su[q] += __shfl_xor(su[q], s, 64);
+                    }
+                    if ((lane & 15) == 0) {
+                        sums[(wm * 2) * HALF + in + q] = sg[q];
+                        sums[(wm * 2 + 1) * HALF + in + q] = su[q];
                     }
                 }
         }
         if (END == End::GATED_GRAD && p.part) {
-            sg += __shfl_xor(sg, 16, 64); sg += __shfl_xor(sg, 32, 64);
-            su += __shfl_xor(su, 16, 64); su += __shfl_xor(su, 32, 64);
-            if (lane < 16) {
-                sums[wm][0][wn * 16 + lane] = sg;
-                sums[wm][1][wn * 16 + lane] = su;
-            }
             __syncthreads();
-            const int c = threadIdx.x % COLS, which = threadIdx.x / COLS;
-            if (which < 2 && n0 + c < p.N)
-                p.part[(int64_t)blockIdx.y * 2 * p.N + which * (int64_t)p.N + n0 + c] =
-                    sums[0][which][c] + sums[1][which][c];
+            for (int c = threadIdx.x; c < 2 * HALF; c += T::THREADS) {
+                const int which = c / HALF, in = c % HALF;
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < T::WM; ++w) s += sums[(w * 2 + which) * HALF + in];
+                if (n0 + in < p.N)
+                    p.part[(int64_t)tm * 2 * p.N + which * (int64_t)p.N + n0 + in] = s;
+            }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < T::MI; ++i) {
+            const int row = row0 + i * 16;
+            if (row >= p.M) continue;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < T::NI; ++j) {
+                const int col = n0 + (wn * T::NI + j) * 16 + (lane >> 4) * 4, have = p.N - col;
+                if (have <= 0) continue;
+                const int64_t at = (int64_t)row * p.N + col;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                if (END == End::PLAIN) {
+                    E out[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int row = m0 + wm * 32 + i * 16 + (lane >> 4) * 4 + q;
-                    const int col = n0 + wn * 32 + j * 16 + (lane & 15);
-                    if (row >= p.M || col >= p.N) continue;
-                    const int64_t at = (int64_t)row * p.N + col;
-                    if (END == End::PLAIN) p.out[at] = from_f<E>(acc[i][j][q]);
-                    else p.part[blockIdx.z * (int64_t)p.M * p.N + at] = acc[i][j][q];
+                    for (int q = 0; q < 4; ++q) out[q] = from_f<E>(v[q]);
+                    store_run<E, 4>(p.out + at, have, out);
+                } else {
+                    store_run<float, 4>(p.part + blockIdx.z * (int64_t)p.M * p.N + at, have, v);
                 }
+            }
+        }
     }
 }
 
@@ -157,71 +363,126 @@ product_kernel(Args<E> p) {
 template <typename E>
 __global__ void __launch_bounds__(256)
 join_splits_kernel(const float* __restrict__ part, E* __restrict__ out, int64_t n, int splits) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
-    float s = 0.0f;
-    for (int z = 0; z < splits; ++z) s += part[z * n + i];
-    out[i] = from_f<E>(s);
+    const int have = n - i < 4 ? (int)(n - i) : 4;
+    float s[4] = {}, v[4];
+    for (int z = 0; z < splits; ++z) {
+        load_run<float, 4>(part + z * n + i, have, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] += v[q];
+    }
+    E o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = from_f<E>(s[q]);
+    store_run<E, 4>(out + i, have, o);
 }
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+using Large = Tile<256, 256, 2, 4>;
+using Small = Tile<128, 128, 2, 2>;
+
+// A tile of 256 x 256 reads half of what four of 128 x 128 do from L2 and LDS,
+// but a card of 256 CUs needs enough of them.
+template <typename E>
+bool large(int64_t m, int64_t n, int splits) {
+    return sizeof(E) == 2 && (int64_t)ceil_div(m, 256) * ceil_div(n, 256) * splits >= 256;
+}
+
+template <typename E, typename T, Lie LA, Lie LB, End END>
+int launch(Args<E> p, int splits, hipStream_t st) {
+    constexpr bool GATED = END == End::GATED || END == End::GATED_GRAD;
+    p.tiles_m = ceil_div(p.M, T::BM);
+    p.tiles_n = ceil_div(p.N, GATED ? T::BN / 2 : T::BN);
+    const dim3 grid(p.tiles_m * p.tiles_n, 1, splits);
+    const auto whole = [](const void* q, int64_t pitch) {
+        return (uintptr_t)q % 16 == 0 && pitch % PIECE<E> == 0;
+    };
+    if (whole(p.a, p.pitch_a) && whole(p.b, p.pitch_b))
+        product_kernel<E, T, LA, LB, END, true><<<grid, T::THREADS, 0, st>>>(p);
+    else
+        product_kernel<E, T, LA, LB, END, false><<<grid, T::THREADS, 0, st>>>(p);
+    LSTM_CHECK_LAUNCH();
+    return 0;
+}
+
+template <typename E, Lie LA, Lie LB, End END>
+int product(const Args<E>& p, int splits, hipStream_t st) {
+    constexpr bool GATED = END == End::GATED || END == End::GATED_GRAD;
+    if constexpr (sizeof(E) == 2)
+        if (large<E>(p.M, GATED ? 2 * (int64_t)p.N : p.N, splits))
+            return launch<E, Large, LA, LB, END>(p, splits, st);
+    return launch<E, Small, LA, LB, END>(p, splits, st);
+}
 
 template <typename E>
 int fwd(const void* x, const void* w, const void* bias, void* y, int M, int K, int F,
         hipStream_t st) {
     if ((int64_t)M * F == 0) return 0;
     Args<E> p{};
-    p.a = (const E*)x; p.am = K; p.ak = 1;
-    p.b = (const E*)w; p.bn = K; p.bk = 1;
+    p.a = (const E*)x; p.pitch_a = K;
+    p.b = (const E*)w; p.pitch_b = K;
     p.M = M; p.N = F; p.K = K; p.per_split = K;
     p.bias = (const E*)bias; p.out = (E*)y;
-    product_kernel<E, End::GATED>
-        <<<dim3(ceil_div(F, TILE / 2), ceil_div(M, TILE)), 256, 0, st>>>(p);
-    LSTM_CHECK_LAUNCH();
-    return 0;
+    return product<E, Lie::K, Lie::K, End::GATED>(p, 1, st);
+}
+
+template <typename E>
+int bias_parts(int M, int F) {
+    return ceil_div(M, large<E>(M, 2 * (int64_t)F, 1) ? Large::BM : Small::BM);
+}
+
+// dw's products run along M, long where its tiles are few: splits of it fill the
+// card, each no shorter than 8 tiles deep.
+template <typename E>
+int splits_of(int M, int K, int F) {
+    const int64_t tiles = (int64_t)ceil_div(2 * (int64_t)F, 128) * ceil_div(K, 128);
+    const int64_t want = ceil_div(512, tiles > 0 ? tiles : 1), most = M / (8 * DEPTH<E>);
+    const int64_t n = want < most ? want : most;
+    return (int)(n > 0 ? n : 1);
 }
 
 template <typename E>
 int bwd(const void* x, const void* w, const void* bias, const void* dy, void* dp, void* dx,
         void* dw, void* db, float* part_db, float* part_dw, int M, int K, int F, int splits,
         hipStream_t st) {
+    int rc = 0;
     if ((int64_t)M * F != 0) {
         Args<E> p{};
-        p.a = (const E*)x; p.am = K; p.ak = 1;
-        p.b = (const E*)w; p.bn = K; p.bk = 1;
+        p.a = (const E*)x; p.pitch_a = K;
+        p.b = (const E*)w; p.pitch_b = K;
         p.M = M; p.N = F; p.K = K; p.per_split = K;
         p.bias = (const E*)bias; p.dy = (const E*)dy; p.out = (E*)dp; p.part = db ? part_db : nullptr;
-        product_kernel<E, End::GATED_GRAD>
-            <<<dim3(ceil_div(F, TILE / 2), ceil_div(M, TILE)), 256, 0, st>>>(p);
-        LSTM_CHECK_LAUNCH();
+        rc = product<E, Lie::K, Lie::K, End::GATED_GRAD>(p, 1, st);
+        if (rc) return rc;
     }
-    if (db) {
-        column_sum_kernel<E><<<ceil_div(2 * F, 64), 1024, 0, st>>>(
-            part_db, (E*)db, ceil_div(M, TILE), 2 * F);
+    if (db && F) {
+        column_sum_kernel<E><<<ceil_div(2 * (int64_t)F, 64), 1024, 0, st>>>(
+            part_db, (E*)db, bias_parts<E>(M, F), 2 * F);
         LSTM_CHECK_LAUNCH();
     }
     if (dx && (int64_t)M * K != 0) {
         Args<E> p{};
-        p.a = (const E*)dp; p.am = 2 * (int64_t)F; p.ak = 1;
-        p.b = (const E*)w; p.bn = 1; p.bk = K;
+        p.a = (const E*)dp; p.pitch_a = 2 * (int64_t)F;
+        p.b = (const E*)w; p.pitch_b = K;
         p.M = M; p.N = K; p.K = 2 * F; p.per_split = 2 * F;
         p.out = (E*)dx;
-        product_kernel<E, End::PLAIN>
-            <<<dim3(ceil_div(K, TILE), ceil_div(M, TILE)), 256, 0, st>>>(p);
-        LSTM_CHECK_LAUNCH();
+        rc = product<E, Lie::K, Lie::INDEX, End::PLAIN>(p, 1, st);
+        if (rc) return rc;
     }
     if (dw && (int64_t)F * K != 0) {
         Args<E> p{};
-        p.a = (const E*)dp; p.am = 1; p.ak = 2 * (int64_t)F;
-        p.b = (const E*)x; p.bn = 1; p.bk = K;
+        p.a = (const E*)dp; p.pitch_a = 2 * (int64_t)F;
+        p.b = (const E*)x; p.pitch_b = K;
         p.M = 2 * F; p.N = K; p.K = M;
-        p.per_split = ceil_div(ceil_div(M > 0 ? M : 1, splits), DEPTH) * DEPTH;
-        p.part = part_dw;
-        product_kernel<E, End::PART>
-            <<<dim3(ceil_div(K, TILE), ceil_div(2 * F, TILE), splits), 256, 0, st>>>(p);
-        LSTM_CHECK_LAUNCH();
+        p.per_split = ceil_div(ceil_div(M > 0 ? M : 1, splits), DEPTH<E>) * DEPTH<E>;
+        p.part = part_dw; p.out = (E*)dw;
+        if (splits == 1) return product<E, Lie::INDEX, Lie::INDEX, End::PLAIN>(p, 1, st);
+        rc = product<E, Lie::INDEX, Lie::INDEX, End::PART>(p, splits, st);
+        if (rc) return rc;
         const int64_t n = (int64_t)2 * F * K;
-        join_splits_kernel<E><<<ceil_div(n, 256), 256, 0, st>>>(part_dw, (E*)dw, n, splits);
+        join_splits_kernel<E><<<ceil_div(n, 1024), 256, 0, st>>>(part_dw, (E*)dw, n, splits);
         LSTM_CHECK_LAUNCH();
     }
     return 0;
@@ -236,12 +497,13 @@ extern "C" int launch_gated_linear_fwd(int is_bf16, const void* x, const void* w
                    : fwd<float>(x, w, bias, y, M, K, F, st);
 }
 
-// Rows of 2F partial sums for db, and splits of 2F * K partial sums for dw.
-extern "C" int gated_linear_bias_parts(int M) { return ceil_div(M, TILE); }
-extern "C" int gated_linear_splits(int M, int K, int F) {
-    const int64_t tiles = (int64_t)ceil_div(2 * F, TILE) * ceil_div(K, TILE);
-    const int64_t want = ceil_div(1024, tiles > 0 ? tiles : 1), most = ceil_div(M, 8 * DEPTH);
-    return (int)(want < most ? (want > 0 ? want : 1) : (most > 0 ? most : 1));
+// Rows of 2F partial sums for db, and splits of 2F * K partial sums for dw (one:
+// none are needed).
+extern "C" int gated_linear_bias_parts(int is_bf16, int M, int F) {
+    return is_bf16 ? bias_parts<bf16>(M, F) : bias_parts<float>(M, F);
+}
+extern "C" int gated_linear_splits(int is_bf16, int M, int K, int F) {
+    return is_bf16 ? splits_of<bf16>(M, K, F) : splits_of<float>(M, K, F);
 }
 
 extern "C" int launch_gated_linear_bwd(int is_bf16, const void* x, const void* w,

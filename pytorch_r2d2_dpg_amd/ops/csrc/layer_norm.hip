@@ -103,16 +103,16 @@ norm_fwd_kernel(const E* __restrict__ x, const E* __restrict__ res,
 // the same from row to row, so the weight's gradient sums up in registers and
 // leaves once a block, as a row of part [gridDim][2][dim].
 //
-// The mean and rstd are computed again from s as it is read: where s is a
-// rounded sum, the forward pass's own belong to other values, and n of a row
-// that hardly varies would be the rounding times a large rstd. The sums join
-// in two rounds: those of s and g, then those of (s - mean)^2 and g (s - mean).
+// s is summed again from x and r, not read back as the forward pass rounded it:
+// in bf16 that rounding alone would add half again to the error of dw. The mean
+// and rstd come from the same registers. The sums join in two rounds: those of
+// s and g, then those of (s - mean)^2 and g (s - mean).
 template <typename E, int TPR, int NV>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
-norm_bwd_kernel(const E* __restrict__ s, const E* __restrict__ w,
-                const E* __restrict__ dy, const E* __restrict__ ds,
-                E* __restrict__ dx, float* __restrict__ part, int64_t rows,
-                int dim, float eps) {
+norm_bwd_kernel(const E* __restrict__ x, const E* __restrict__ res,
+                const E* __restrict__ w, const E* __restrict__ dy,
+                const E* __restrict__ ds, E* __restrict__ dx,
+                float* __restrict__ part, int64_t rows, int dim, float eps) {
     constexpr int R = RUN<E>;
     constexpr int ROWS = TPR > 256 ? 1 : 256 / TPR;
     __shared__ float lds[16];
@@ -125,16 +125,17 @@ norm_bwd_kernel(const E* __restrict__ s, const E* __restrict__ w,
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (tid + k * TPR) * R, have = dim - c;
-            E sin[R], din[R], win[R];
+            E xin[R], rin[R], din[R], win[R];
             if (have > 0) {
-                load_run<E, R>(s + row * dim + c, have, sin);
+                load_run<E, R>(x + row * dim + c, have, xin);
+                if (res) load_run<E, R>(res + row * dim + c, have, rin);
                 load_run<E, R>(dy + row * dim + c, have, din);
                 load_run<E, R>(w + c, have, win);
             }
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const bool real = i < have;
-                n[k][i] = real ? to_f(sin[i]) : 0.0f;
+                n[k][i] = real ? to_f(xin[i]) + (res ? to_f(rin[i]) : 0.0f) : 0.0f;
                 d[k][i] = real ? to_f(din[i]) : 0.0f;
                 g[k][i] = real ? d[k][i] * to_f(win[i]) : 0.0f;
                 sum += n[k][i];
@@ -235,21 +236,21 @@ norm_fwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
 // norm_dw_long_kernel.
 template <typename E>
 __global__ void __launch_bounds__(1024)
-norm_bwd_long_kernel(const E* __restrict__ s, const E* __restrict__ w,
-                     float* __restrict__ stats, const E* __restrict__ dy,
+norm_bwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
+                     const E* __restrict__ w, float* __restrict__ stats, const E* __restrict__ dy,
                      const E* __restrict__ ds, E* __restrict__ dx, int dim, float eps) {
     __shared__ float lds[16];
     const int64_t row = blockIdx.x;
-    const E *sr = s + row * dim, *dr = dy + row * dim;
+    const E *xr = x + row * dim, *rr = res ? res + row * dim : nullptr, *dr = dy + row * dim;
     float sum = 0.0f, sg = 0.0f, sq = 0.0f, sgn = 0.0f;
     for (int c = threadIdx.x; c < dim; c += 1024) {
-        sum += to_f(sr[c]);
+        sum += to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
         sg += to_f(dr[c]) * to_f(w[c]);
     }
     const float mean = row_sum<1024>(sum, lds) / dim;
     sg = row_sum<1024>(sg, lds) / dim;
     for (int c = threadIdx.x; c < dim; c += 1024) {
-        const float n = to_f(sr[c]) - mean;
+        const float n = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean;
         sq += n * n;
         sgn += to_f(dr[c]) * to_f(w[c]) * n;
     }
@@ -261,7 +262,7 @@ norm_bwd_long_kernel(const E* __restrict__ s, const E* __restrict__ w,
     }
     for (int c = threadIdx.x; c < dim; c += 1024) {
         const float g = to_f(dr[c]) * to_f(w[c]);
-        const float n = (to_f(sr[c]) - mean) * rstd;
+        const float n = (to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean) * rstd;
         dx[row * dim + c] = from_f<E>((g - sg - n * sgn) * rstd +
                                       (ds ? to_f(ds[row * dim + c]) : 0.0f));
     }
@@ -269,15 +270,16 @@ norm_bwd_long_kernel(const E* __restrict__ s, const E* __restrict__ w,
 
 template <typename E>
 __global__ void __launch_bounds__(256)
-norm_dw_long_kernel(const E* __restrict__ s, const float* __restrict__ stats,
-                    const E* __restrict__ dy, float* __restrict__ part,
+norm_dw_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
+                    const float* __restrict__ stats, const E* __restrict__ dy, float* __restrict__ part,
                     int64_t rows, int dim) {
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= dim) return;
     float dw = 0.0f, db = 0.0f;
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const float d = to_f(dy[row * dim + c]);
-        dw += d * (to_f(s[row * dim + c]) - stats[2 * row]) * stats[2 * row + 1];
+        const float v = to_f(x[row * dim + c]) + (res ? to_f(res[row * dim + c]) : 0.0f);
+        dw += d * (v - stats[2 * row]) * stats[2 * row + 1];
         db += d;
     }
     part[((int64_t)blockIdx.y * 2) * dim + c] = dw;
@@ -332,21 +334,23 @@ int fwd(const void* x, const void* res, const void* w, const void* b, void* y,
 }
 
 template <typename E>
-int bwd(const void* s, const void* w, const void* dy, const void* ds, void* dx, float* part,
-        float* stats, void* dwb, int64_t rows, int dim, int parts, float eps, hipStream_t st) {
+int bwd(const void* x, const void* res, const void* w, const void* dy, const void* ds, void* dx,
+        float* part, float* stats, void* dwb, int64_t rows, int dim, int parts, float eps, hipStream_t st) {
     if (rows == 0) {
         parts = 0;
     } else if (shape_of<E>(dim).threads == 0) {
         norm_bwd_long_kernel<E><<<dim3((unsigned)rows), 1024, 0, st>>>(
-            (const E*)s, (const E*)w, stats, (const E*)dy, (const E*)ds, (E*)dx, dim, eps);
+            (const E*)x, (const E*)res, (const E*)w, stats, (const E*)dy, (const E*)ds, (E*)dx, dim,
+            eps);
         LSTM_CHECK_LAUNCH();
         norm_dw_long_kernel<E><<<dim3((dim + 255) / 256, parts), 256, 0, st>>>(
-            (const E*)s, stats, (const E*)dy, part, rows, dim);
+            (const E*)x, (const E*)res, stats, (const E*)dy, part, rows, dim);
     } else {
         with_shape<E>(dim, [&](auto t, auto n) {
             constexpr int T = decltype(t)::value, N = decltype(n)::value;
             norm_bwd_kernel<E, T, N><<<parts, T > 256 ? T : 256, 0, st>>>(
-                (const E*)s, (const E*)w, (const E*)dy, (const E*)ds, (E*)dx, part, rows, dim, eps);
+                (const E*)x, (const E*)res, (const E*)w, (const E*)dy, (const E*)ds, (E*)dx, part,
+                rows, dim, eps);
         });
     }
     LSTM_CHECK_LAUNCH();
@@ -377,10 +381,11 @@ extern "C" int64_t norm_bwd_stats(int is_bf16, int64_t rows, int dim) {
     return p.threads ? 0 : 2 * rows;
 }
 
-extern "C" int launch_norm_bwd(int is_bf16, const void* s, const void* w, const void* dy,
-                               const void* ds, void* dx, float* part, float* stats, void* dwb,
-                               int64_t rows, int dim, int parts, float eps, hipStream_t st) {
+extern "C" int launch_norm_bwd(int is_bf16, const void* x, const void* res, const void* w,
+                               const void* dy, const void* ds, void* dx, float* part,
+                               float* stats, void* dwb, int64_t rows, int dim, int parts,
+                               float eps, hipStream_t st) {
     return is_bf16
-        ? bwd<bf16>(s, w, dy, ds, dx, part, stats, dwb, rows, dim, parts, eps, st)
-        : bwd<float>(s, w, dy, ds, dx, part, stats, dwb, rows, dim, parts, eps, st);
+        ? bwd<bf16>(x, res, w, dy, ds, dx, part, stats, dwb, rows, dim, parts, eps, st)
+        : bwd<float>(x, res, w, dy, ds, dx, part, stats, dwb, rows, dim, parts, eps, st);
 }

@@ -24,18 +24,16 @@ class _LayerNorm(torch.autograd.Function):
         y, s = hip_ext().layer_norm_fwd(x, weight, bias, residual, eps)
         ctx.set_materialize_grads(False)
         ctx.has_bias, ctx.fused, ctx.eps = bias is not None, residual is not None, eps
-        # The backward pass takes s as it was rounded to the inputs' type, and
-        # the statistics of that: half a step of s, as any op that keeps its input.
-        ctx.save_for_backward(x if residual is None else s, weight)
+        ctx.save_for_backward(x, weight, residual)
         return y if residual is None else (y, s)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, ds=None):
-        s, weight = ctx.saved_tensors
-        dy = torch.zeros_like(s) if dy is None else dy.contiguous()
+        x, weight, residual = ctx.saved_tensors
+        dy = torch.zeros_like(x) if dy is None else dy.contiguous()
         ds = None if ds is None else ds.contiguous()
-        dx, dwb = hip_ext().layer_norm_bwd(s, weight, dy, ds, ctx.eps)
+        dx, dwb = hip_ext().layer_norm_bwd(x, residual, weight, dy, ds, ctx.eps)
         return dx, dwb[0], dwb[1] if ctx.has_bias else None, dx if ctx.fused else None, None
 
 

@@ -61,12 +61,6 @@ def norm_oracle(x, w, b, r, dy, ds, eps=1e-5):
         res = [(y.detach(), ey)]
         if r is not None:
             res.append((s.detach(), (h + 2 * U) * s.abs()))
-            # Backward reads the rounded s and its own statistics: to first order
-            # n moves by rstd (d - mean(d) - n mean(n d)), rstd by rstd^2 mean(n d).
-            d = h * s.abs()
-            shift = rstd * (n.abs() * d).mean(-1, keepdim=True)
-            en = en + rstd * (d + d.mean(-1, keepdim=True)) + n.abs() * shift
-            er = er + shift
         g = dy * w
         gn, eg = (g * n).mean(-1, keepdim=True), 2 * U * g.abs()
         egn = (g.abs() * en + eg * n.abs() + SUM * U * (g * n).abs()).mean(-1, keepdim=True)

@@ -261,7 +261,7 @@ def test_linear_widths(K, F, dtype):
     run_linear(70, K, F, dtype, bias=F != 16, seed=K + F)
 
 
-@pytest.mark.parametrize("M, K, F", [(1500, 512, 1024), (5000, 96, 64), (33, 2048, 512)])
+@pytest.mark.parametrize("M, K, F", [(1500, 512, 1024), (5000, 96, 64), (33, 2048, 512), (8200, 136, 1032), (8195, 67, 1029)])
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_linear_larger(M, K, F, dtype):
     run_linear(M, K, F, dtype, seed=M)
