@@ -14,7 +14,7 @@ template <> DEV_INLINE float from_f<float>(float v) { return v; }
 template <> DEV_INLINE bf16 from_f<bf16>(float v) { return f2bf(v); }
 
 // sigma(x) and sigma(-x) = 1 - sigma(x) from one exponential of -|x|: neither
-// cancels where the other is near one. The exp2 and rcp instructions are within
+// cancels where the other is near one, and a NaN is both. The exp2 and rcp instructions are within
 // 1 ulp, the argument's rounding adds |x| * 2^-24.
 DEV_INLINE void sigmoid_pair(float x, float& pos, float& neg) {
     const float e = __builtin_amdgcn_exp2f(-fabsf(x) * 1.44269504f);
@@ -22,7 +22,6 @@ DEV_INLINE void sigmoid_pair(float x, float& pos, float& neg) {
     const float small = e * big;
     pos = x >= 0.0f ? big : small;
     neg = x >= 0.0f ? small : big;
-    if (x != x) pos = neg = x;
 }
 
 // silu(x) = x * sigma(x) and its derivative sigma + x sigma (1 - sigma).
@@ -66,6 +65,25 @@ DEV_INLINE void store_run(E* p, int have, const E (&in)[N]) {
             if (i < have) p[i] = in[i];
     }
 }
+
+// Two values as they lie in memory; a register of two bf16 until they are used.
+template <typename E> struct Two;
+template <> struct Two<float> {
+    float v[2];
+    DEV_INLINE float operator[](int i) const { return v[i]; }
+    static DEV_INLINE Two of(float a, float b) { return {{a, b}}; }
+};
+template <> struct Two<bf16> {
+    unsigned v;
+    DEV_INLINE float operator[](int i) const {
+        return __uint_as_float(i ? v & 0xffff0000u : v << 16);
+    }
+    static DEV_INLINE Two of(float a, float b) {
+        using f2 = __attribute__((ext_vector_type(2))) float;
+        using b2 = __attribute__((ext_vector_type(2))) __bf16;
+        return {__builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2))};
+    }
+};
 
 DEV_INLINE float wave_sum(float v) {
 #pragma unroll

@@ -24,7 +24,7 @@
 
 namespace {
 
-constexpr int CHUNK = 16;  // steps of a wave, and between two kept states
+constexpr int CHUNK = 8;  // steps of a wave, and between two kept states
 constexpr int MAX_WAVES = 8;
 
 template <typename E>
@@ -44,40 +44,54 @@ struct Args {
 };
 
 // A lane's channels: the pair (c, c + 1) of a row b; the last of an odd H alone.
+// A lane past the end has n = 0 and reads what the last one does.
 struct Lane {
-    int b, c, n, len;  // n: 0 past the end, else 1 or 2
+    int b, c, n, len;
 };
 
 template <typename E>
 DEV_INLINE Lane lane_of(const Args<E>& p) {
     const int pairs = (p.H + 1) / 2;
-    const int64_t u = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    Lane q{0, 0, 0, 0};
-    if (u < (int64_t)pairs * p.B) {
-        q.b = (int)(u / pairs);
-        q.c = 2 * (int)(u - (int64_t)q.b * pairs);
-        q.n = q.c + 1 < p.H ? 2 : 1;
-        q.len = p.T;
-        if (p.lengths) {
-            const int len = p.lengths[q.b];
-            q.len = len < 0 ? 0 : len > p.T ? p.T : len;
-        }
+    const int64_t units = (int64_t)pairs * p.B;
+    int64_t u = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    const bool in = u < units;
+    if (!in) u = units - 1;
+    Lane q;
+    q.b = (int)(u / pairs);
+    q.c = 2 * (int)(u - (int64_t)q.b * pairs);
+    q.n = !in ? 0 : q.c + 1 < p.H ? 2 : 1;
+    q.len = p.T;
+    if (p.lengths) {
+        const int len = p.lengths[q.b];
+        q.len = len < 0 ? 0 : len > p.T ? p.T : len;
     }
     return q;
 }
 
-template <typename E>
-DEV_INLINE void load2(const E* p, int n, E (&out)[2]) {
-    load_run<E, 2>(p, n, out);
+// Two elements without a branch, which would keep the loads behind it waiting:
+// `second` is 0 where a lane has one channel.
+template <bool EVEN, typename E>
+DEV_INLINE Two<E> load2(const E* p, int second) {
+    struct __attribute__((packed, aligned(sizeof(E)))) Raw { Two<E> v; };
+    if constexpr (EVEN) {
+        return reinterpret_cast<const Raw*>(p)->v;
+    } else {
+        const E e[2] = {p[0], p[second]};
+        return __builtin_bit_cast(Two<E>, e);
+    }
 }
 
-DEV_INLINE void load_state(const float* p, const Lane& q, int H, float (&h)[2]) {
-    h[0] = h[1] = 0.0f;
-    if (p && q.n) load_run<float, 2>(p + (int64_t)q.b * H + q.c, q.n, h);
-}
-
-DEV_INLINE void store_state(float* p, const Lane& q, int H, const float (&h)[2]) {
-    if (q.n) store_run<float, 2>(p + (int64_t)q.b * H + q.c, q.n, h);
+template <bool EVEN, typename E>
+DEV_INLINE void store2(E* p, int n, float a, float b) {
+    struct __attribute__((packed, aligned(sizeof(E)))) Raw { Two<E> v; };
+    const Two<E> v = Two<E>::of(a, b);
+    if constexpr (EVEN) {
+        if (n) reinterpret_cast<Raw*>(p)->v = v;
+    } else {
+        const Run<E, 2> e = __builtin_bit_cast(Run<E, 2>, v);
+        if (n) p[0] = e.v[0];
+        if (n > 1) p[1] = e.v[1];
+    }
 }
 
 // The waves' maps meet in LDS. `carry` is the state before the block's first
@@ -125,55 +139,54 @@ DEV_INLINE void join_segments(const Args<E>& p, const Lane& q, int seg, float (&
 }
 
 // ONLY_MAP: leave the segment's map and write nothing else.
-template <typename E, bool ONLY_MAP>
+template <typename E, bool EVEN, bool ONLY_MAP>
 __global__ void __launch_bounds__(64 * MAX_WAVES)
 recurrence_fwd_kernel(Args<E> p) {
     __shared__ float2 slots[2][MAX_WAVES][64][2];
     const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, seg = blockIdx.y;
     const Lane q = lane_of(p);
+    const int second = q.c + 1 < p.H;
     const int64_t step = (int64_t)p.B * p.H;
     const int64_t at = (int64_t)q.b * p.H + q.c;
+    const E* lane_gates = p.gates + 3 * (int64_t)q.b * p.H + q.c;
     float carry[2] = {0.0f, 0.0f}, total[2] = {1.0f, 1.0f};
     if (!ONLY_MAP) {
-        load_state(p.h0, q, p.H, carry);
+        if (p.h0) {
+            const Two<float> s = load2<EVEN>(p.h0 + at, second);
+            carry[0] = s[0];
+            carry[1] = s[1];
+        }
         join_segments<false>(p, q, seg, carry);
     }
     int turn = 0;
     for (int pass = 0; pass < p.passes; ++pass) {
         const int chunk = (seg * p.passes + pass) * waves + wave;
         const int t0 = chunk * CHUNK;
+        // every load of the chunk first: the branches are the wave's, not a lane's
+        Two<E> f[CHUNK], v[CHUNK], o[CHUNK];
+#pragma unroll
+        for (int k = 0; k < CHUNK; ++k)
+            if (t0 + k < p.T) {
+                const E* g = lane_gates + 3 * (t0 + k) * step;
+                f[k] = load2<EVEN>(g, second);
+                v[k] = load2<EVEN>(g + p.H, second);
+                if (!ONLY_MAP) o[k] = load2<EVEN>(g + 2 * (int64_t)p.H, second);
+            }
         float a[CHUNK][2], b[CHUNK][2];
-        E o[CHUNK][2];
-#pragma unroll
-        for (int k = 0; k < CHUNK; ++k) {
-            const int t = t0 + k;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[k][i] = 1.0f;
-                b[k][i] = 0.0f;
-                o[k][i] = from_f<E>(0.0f);
-            }
-            if (t < q.len) {  // len is 0 for a lane past the end
-                const E* g = p.gates + 3 * (int64_t)t * step + 3 * (int64_t)q.b * p.H + q.c;
-                E f[2], v[2];
-                load2(g, q.n, f);
-                load2(g + p.H, q.n, v);
-                if (!ONLY_MAP) load2(g + 2 * (int64_t)p.H, q.n, o[k]);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float keep;
-                    sigmoid_pair(to_f(f[i]), a[k][i], keep);
-                    b[k][i] = keep * to_f(v[i]);
-                }
-            }
-        }
         float A[2] = {1.0f, 1.0f}, Hl[2] = {0.0f, 0.0f}, h[2];
 #pragma unroll
         for (int k = 0; k < CHUNK; ++k)
+            if (t0 + k < p.T) {
+                const bool real = t0 + k < q.len;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                Hl[i] = a[k][i] * Hl[i] + b[k][i];
-                A[i] *= a[k][i];
+                for (int i = 0; i < 2; ++i) {
+                    float pos, neg;
+                    sigmoid_pair(f[k][i], pos, neg);
+                    a[k][i] = real ? pos : 1.0f;
+                    b[k][i] = real ? neg * v[k][i] : 0.0f;
+                    Hl[i] = a[k][i] * Hl[i] + b[k][i];
+                    A[i] *= a[k][i];
+                }
             }
         if (waves > 1) {
             join_waves<false>(slots, turn, wave, waves, A, Hl, carry, h);
@@ -191,102 +204,101 @@ recurrence_fwd_kernel(Args<E> p) {
             }
         }
         if (ONLY_MAP) continue;
-        if (p.kept && t0 < p.T && q.n)
-            store_run<float, 2>(p.kept + chunk * step + at, q.n, h);
+        if (p.kept && t0 < p.T) store2<EVEN>(p.kept + chunk * step + at, q.n, h[0], h[1]);
 #pragma unroll
-        for (int k = 0; k < CHUNK; ++k) {
-            const int t = t0 + k;
-            if (t >= p.T) break;
-            E out[2];
+        for (int k = 0; k < CHUNK; ++k)
+            if (t0 + k < p.T) {
+                const bool real = t0 + k < q.len;
+                float out[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                h[i] = a[k][i] * h[i] + b[k][i];
-                float val, grad;
-                silu_grad(to_f(o[k][i]), val, grad);
-                out[i] = from_f<E>(t < q.len ? h[i] * val : 0.0f);
+                for (int i = 0; i < 2; ++i) {
+                    h[i] = a[k][i] * h[i] + b[k][i];
+                    float val, grad;
+                    silu_grad(o[k][i], val, grad);
+                    out[i] = real ? h[i] * val : 0.0f;
+                }
+                store2<EVEN>(p.y + (t0 + k) * step + at, q.n, out[0], out[1]);
             }
-            if (q.n) store_run<E, 2>(p.y + t * step + at, q.n, out);
-        }
     }
+    if (wave != 0) return;
     if (ONLY_MAP) {
-        if (wave == 0)
-            for (int i = 0; i < q.n; ++i)
-                p.maps[seg * step + at + i] = make_float2(total[i], carry[i]);
-    } else if (wave == 0 && seg == p.segments - 1) {
-        store_state(p.hT, q, p.H, carry);
+        for (int i = 0; i < q.n; ++i)
+            p.maps[seg * step + at + i] = make_float2(total[i], carry[i]);
+    } else if (seg == p.segments - 1) {
+        store2<EVEN>(p.hT + at, q.n, carry[0], carry[1]);
     }
 }
 
 // R_t = a_t G_t is what step t hands to step t - 1, and the map of a step is
 // R -> a (R + p) with p = dy silu(o).
-template <typename E, bool ONLY_MAP>
+template <typename E, bool EVEN, bool ONLY_MAP>
 __global__ void __launch_bounds__(64 * MAX_WAVES)
 recurrence_bwd_kernel(Args<E> p) {
     __shared__ float2 slots[2][MAX_WAVES][64][2];
     const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, seg = blockIdx.y;
     const Lane q = lane_of(p);
+    const int second = q.c + 1 < p.H;
     const int64_t step = (int64_t)p.B * p.H;
-    const int64_t at = (int64_t)q.b * p.H + q.c;
+    const int64_t at = (int64_t)q.b * p.H + q.c, gate_at = 3 * (int64_t)q.b * p.H + q.c;
     float carry[2] = {0.0f, 0.0f}, total[2] = {1.0f, 1.0f};
     if (!ONLY_MAP) {
-        load_state(p.dhT, q, p.H, carry);
+        if (p.dhT) {
+            const Two<float> s = load2<EVEN>(p.dhT + at, second);
+            carry[0] = s[0];
+            carry[1] = s[1];
+        }
         join_segments<true>(p, q, seg, carry);
     }
     int turn = 0;
     for (int pass = p.passes - 1; pass >= 0; --pass) {
         const int chunk = (seg * p.passes + pass) * waves + wave;
         const int t0 = chunk * CHUNK;
+        Two<E> f[CHUNK], v[CHUNK], o[CHUNK], dy[CHUNK];
+        Two<float> h{};
+        if (!ONLY_MAP && t0 < p.T) h = load2<EVEN>(p.kept + chunk * step + at, second);
+#pragma unroll
+        for (int k = 0; k < CHUNK; ++k)
+            if (t0 + k < p.T) {
+                const E* g = p.gates + 3 * (t0 + k) * step + gate_at;
+                f[k] = load2<EVEN>(g, second);
+                if (!ONLY_MAP) v[k] = load2<EVEN>(g + p.H, second);
+                o[k] = load2<EVEN>(g + 2 * (int64_t)p.H, second);
+                dy[k] = load2<EVEN>(p.dy + (t0 + k) * step + at, second);
+            }
         // Of a and 1 - a the smaller is held, with the sign saying which: the
         // other follows without cancelling, in half the registers.
         float m[CHUNK][2], before[CHUNK][2], g[CHUNK][2];
-        E v[CHUNK][2];
-        float h[2] = {0.0f, 0.0f};
-        if (!ONLY_MAP && t0 < p.T && q.n) load_run<float, 2>(p.kept + chunk * step + at, q.n, h);
 #pragma unroll
-        for (int k = 0; k < CHUNK; ++k) {
-            const int t = t0 + k;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                m[k][i] = -0.0f;  // a = 1
-                g[k][i] = 0.0f;
-                before[k][i] = 0.0f;
-                v[k][i] = from_f<E>(0.0f);
-            }
-            E dout[2] = {from_f<E>(0.0f), from_f<E>(0.0f)};
-            const int64_t gate = 3 * (int64_t)t * step + 3 * (int64_t)q.b * p.H + q.c;
-            if (t < q.len) {
-                const E* gp = p.gates + gate;
-                E f[2], o[2], dy[2];
-                load2(gp, q.n, f);
-                if (!ONLY_MAP) load2(gp + p.H, q.n, v[k]);
-                load2(gp + 2 * (int64_t)p.H, q.n, o);
-                load2(p.dy + t * step + at, q.n, dy);
+        for (int k = 0; k < CHUNK; ++k)
+            if (t0 + k < p.T) {
+                const bool real = t0 + k < q.len;
+                float out[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float a, keep, val, grad;
-                    sigmoid_pair(to_f(f[i]), a, keep);
-                    silu_grad(to_f(o[i]), val, grad);
-                    m[k][i] = a <= keep ? a : -keep;
-                    g[k][i] = to_f(dy[i]) * val;
+                    sigmoid_pair(f[k][i], a, keep);
+                    silu_grad(o[k][i], val, grad);
+                    m[k][i] = real ? (a <= keep ? a : -keep) : -0.0f;  // a pad: a = 1
+                    g[k][i] = real ? dy[k][i] * val : 0.0f;
                     if (!ONLY_MAP) {
                         before[k][i] = h[i];
-                        h[i] = a * h[i] + keep * to_f(v[k][i]);
-                        dout[i] = from_f<E>(to_f(dy[i]) * h[i] * grad);
+                        h.v[i] = real ? a * h[i] + keep * v[k][i] : h[i];
+                        out[i] = real ? dy[k][i] * h[i] * grad : 0.0f;
                     }
                 }
+                if (!ONLY_MAP)
+                    store2<EVEN>(p.dgates + 3 * (t0 + k) * step + gate_at + 2 * (int64_t)p.H, q.n, out[0], out[1]);
             }
-            if (!ONLY_MAP && t < p.T && q.n)
-                store_run<E, 2>(p.dgates + gate + 2 * (int64_t)p.H, q.n, dout);
-        }
         float A[2] = {1.0f, 1.0f}, Rl[2] = {0.0f, 0.0f}, R[2];
 #pragma unroll
         for (int k = CHUNK - 1; k >= 0; --k)
+            if (t0 + k < p.T)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float a = __builtin_signbit(m[k][i]) ? 1.0f + m[k][i] : m[k][i];
-                Rl[i] = a * (Rl[i] + g[k][i]);
-                A[i] *= a;
-            }
+                for (int i = 0; i < 2; ++i) {
+                    const float a = __builtin_signbit(m[k][i]) ? 1.0f + m[k][i] : m[k][i];
+                    Rl[i] = a * (Rl[i] + g[k][i]);
+                    A[i] *= a;
+                }
         if (waves > 1) {
             join_waves<true>(slots, turn, wave, waves, A, Rl, carry, R);
             if (ONLY_MAP)
@@ -304,34 +316,31 @@ recurrence_bwd_kernel(Args<E> p) {
         }
         if (ONLY_MAP) continue;
 #pragma unroll
-        for (int k = CHUNK - 1; k >= 0; --k) {
-            const int t = t0 + k;
-            if (t >= p.T) continue;
-            E df[2], dv[2];
+        for (int k = CHUNK - 1; k >= 0; --k)
+            if (t0 + k < p.T) {
+                const bool real = t0 + k < q.len;
+                float df[2], dv[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool neg = __builtin_signbit(m[k][i]);
-                const float a = neg ? 1.0f + m[k][i] : m[k][i];
-                const float keep = neg ? -m[k][i] : 1.0f - m[k][i];
-                const float G = R[i] + g[k][i];
-                R[i] = a * G;
-                const bool real = t < q.len;
-                df[i] = from_f<E>(real ? R[i] * keep * (before[k][i] - to_f(v[k][i])) : 0.0f);
-                dv[i] = from_f<E>(real ? G * keep : 0.0f);
+                for (int i = 0; i < 2; ++i) {
+                    const bool neg = __builtin_signbit(m[k][i]);
+                    const float a = neg ? 1.0f + m[k][i] : m[k][i];
+                    const float keep = neg ? -m[k][i] : 1.0f - m[k][i];
+                    const float G = R[i] + g[k][i];
+                    R[i] = a * G;
+                    df[i] = real ? R[i] * keep * (before[k][i] - v[k][i]) : 0.0f;
+                    dv[i] = real ? G * keep : 0.0f;
+                }
+                E* to = p.dgates + 3 * (t0 + k) * step + gate_at;
+                store2<EVEN>(to, q.n, df[0], df[1]);
+                store2<EVEN>(to + p.H, q.n, dv[0], dv[1]);
             }
-            if (q.n) {
-                E* gp = p.dgates + 3 * (int64_t)t * step + 3 * (int64_t)q.b * p.H + q.c;
-                store_run<E, 2>(gp, q.n, df);
-                store_run<E, 2>(gp + p.H, q.n, dv);
-            }
-        }
     }
+    if (wave != 0) return;
     if (ONLY_MAP) {
-        if (wave == 0)
-            for (int i = 0; i < q.n; ++i)
-                p.maps[seg * step + at + i] = make_float2(total[i], carry[i]);
-    } else if (wave == 0 && seg == 0) {
-        store_state(p.dh0, q, p.H, carry);
+        for (int i = 0; i < q.n; ++i)
+            p.maps[seg * step + at + i] = make_float2(total[i], carry[i]);
+    } else if (seg == 0) {
+        store2<EVEN>(p.dh0 + at, q.n, carry[0], carry[1]);
     }
 }
 
@@ -343,7 +352,8 @@ struct Plan {
 };
 
 Plan plan_of(int T, int B, int H) {
-    const int chunks = T > 0 ? (T + CHUNK - 1) / CHUNK : 1;
+    if (T == 0) return {1, 1, 0};  // the state alone
+    const int chunks = (T + CHUNK - 1) / CHUNK;
     const int64_t tiles = ((int64_t)B * ((H + 1) / 2) + 63) / 64;
     int passes = (chunks + MAX_WAVES - 1) / MAX_WAVES;
     const int waves = (chunks + passes - 1) / passes;
@@ -365,16 +375,19 @@ int run(Args<E> p, bool back, hipStream_t st) {
     p.passes = plan.passes;
     const int64_t tiles = ((int64_t)p.B * ((p.H + 1) / 2) + 63) / 64;
     const dim3 grid((unsigned)tiles, plan.segments), block(64 * plan.waves);
+    const auto go = [&](auto even, auto only_map) {
+        constexpr bool EVEN = decltype(even)::value, MAP = decltype(only_map)::value;
+        if (back) recurrence_bwd_kernel<E, EVEN, MAP><<<grid, block, 0, st>>>(p);
+        else recurrence_fwd_kernel<E, EVEN, MAP><<<grid, block, 0, st>>>(p);
+        return hipGetLastError() == hipSuccess;
+    };
+    const std::true_type yes;
+    const std::false_type no;
     if (plan.segments > 1) {
         if (!p.maps) return -1;
-        if (back) recurrence_bwd_kernel<E, true><<<grid, block, 0, st>>>(p);
-        else recurrence_fwd_kernel<E, true><<<grid, block, 0, st>>>(p);
-        LSTM_CHECK_LAUNCH();
+        if (!(p.H % 2 ? go(no, yes) : go(yes, yes))) return -3;
     }
-    if (back) recurrence_bwd_kernel<E, false><<<grid, block, 0, st>>>(p);
-    else recurrence_fwd_kernel<E, false><<<grid, block, 0, st>>>(p);
-    LSTM_CHECK_LAUNCH();
-    return 0;
+    return (p.H % 2 ? go(no, no) : go(yes, no)) ? 0 : -3;
 }
 
 template <typename E>
