@@ -119,7 +119,8 @@ std::tuple<Tensor, Tensor, Tensor> gated_recurrence_fwd(Tensor gates, OptTensor 
     TORCH_CHECK(gates.dim() == 3 && gates.size(2) % 3 == 0, "gates must be [T, B, 3H]");
     const c10::DeviceGuard guard(gates.device());
     const int64_t T = gates.size(0), B = gates.size(1), H = gates.size(2) / 3;
-    TORCH_CHECK(T <= MOST && B * (H + 1) <= MOST * 64 && B <= MOST && H <= MOST,
+    // places in a step are counted in 32 bits, of the whole in 64
+    TORCH_CHECK(T <= MOST && B <= MOST && H <= MOST && 3 * B * (H + 1) <= MOST,
                 "gates is too large");
     if (h0) check(*h0, "h0", gates, torch::kFloat32, {B, H});
     if (lengths) check(*lengths, "lengths", gates, torch::kInt32, {B});
