@@ -4,6 +4,7 @@
 #include "common.h"
 
 #include <cstdint>
+#include <type_traits>
 
 using bf16 = __hip_bfloat16;
 
@@ -85,31 +86,64 @@ template <> struct Two<bf16> {
     }
 };
 
+// Sum over a wave, the same in each lane: four steps inside rows of 16 lanes as
+// operands of the additions, two across rows by lane swaps, none through LDS.
 DEV_INLINE float wave_sum(float v) {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
+#ifdef __HIP_DEVICE_COMPILE__
+    const auto turned = [](float x, auto control) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x),
+                                                          decltype(control)::value, 0xf, 0xf, true));
+    };
+    v += turned(v, std::integral_constant<int, 0xb1>());   // lane ^ 1
+    v += turned(v, std::integral_constant<int, 0x4e>());   // lane ^ 2
+    v += turned(v, std::integral_constant<int, 0x141>());  // half a row mirrored
+    v += turned(v, std::integral_constant<int, 0x140>());  // a row mirrored
+    const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v),
+                                                       false, false);
+    v = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
+                                                         false, false);
+    v = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+#endif
     return v;
 }
 
-// out[c] = sum over r of part[r][c], rows in a fixed order: the second stage of
-// a reduction over rows, in place of atomics whose order would change results.
-// 16 waves share 64 columns, wave w the rows w, w+16, ...
+// out[c] = sum over r of part[r][c] in a fixed order: the second stage of a
+// reduction over rows, in place of atomics whose order would change results.
+// A block has 16 columns, which 64 groups of threads walk 64 rows apart, eight
+// loads at a time.
 template <typename E>
 static __global__ void __launch_bounds__(1024)
 column_sum_kernel(const float* __restrict__ part, E* __restrict__ out,
                   int rows, int cols) {
-    __shared__ float sums[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane;
+    __shared__ float sums[64][17];
+    const int in = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + in;
+    const float* p = part + (c < cols ? c : cols - 1);
     float s = 0.0f;
-    if (c < cols)
-        for (int r = wave; r < rows; r += 16) s += part[(int64_t)r * cols + c];
-    sums[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && c < cols) {
-        float t = 0.0f;
+    for (int r0 = group; r0 < rows; r0 += 8 * 64) {
+        float v[8];
 #pragma unroll
-        for (int w = 0; w < 16; ++w) t += sums[w][lane];
-        out[c] = from_f<E>(t);
+        for (int k = 0; k < 8; ++k) {
+            const int r = r0 + 64 * k;
+            v[k] = p[(int64_t)(r < rows ? r : rows - 1) * cols];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += r0 + 64 * k < rows ? v[k] : 0.0f;
     }
+    sums[group][in] = s;
+    __syncthreads();
+    if (threadIdx.x < 16 && c < cols) {
+        float t[4] = {};
+#pragma unroll
+        for (int g = 0; g < 64; ++g) t[g & 3] += sums[g][in];
+        out[c] = from_f<E>((t[0] + t[1]) + (t[2] + t[3]));
+    }
+}
+
+template <typename E>
+static int column_sum(const float* part, E* out, int rows, int cols, hipStream_t st) {
+    if (cols) column_sum_kernel<E><<<(cols + 15) / 16, 1024, 0, st>>>(part, out, rows, cols);
+    LSTM_CHECK_LAUNCH();
+    return 0;
 }

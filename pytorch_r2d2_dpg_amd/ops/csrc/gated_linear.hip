@@ -458,9 +458,8 @@ int bwd(const void* x, const void* w, const void* bias, const void* dy, void* dp
         if (rc) return rc;
     }
     if (db && F) {
-        column_sum_kernel<E><<<ceil_div(2 * (int64_t)F, 64), 1024, 0, st>>>(
-            part_db, (E*)db, bias_parts<E>(M, F), 2 * F);
-        LSTM_CHECK_LAUNCH();
+        rc = column_sum<E>(part_db, (E*)db, bias_parts<E>(M, F), 2 * F, st);
+        if (rc) return rc;
     }
     if (dx && (int64_t)M * K != 0) {
         Args<E> p{};

@@ -11,165 +11,206 @@
 
 namespace {
 
-constexpr int BYTES = 16;  // one load of a lane
+template <typename E> constexpr int RUN = 16 / (int)sizeof(E);  // one load of a lane
 
-template <typename E> constexpr int RUN = BYTES / (int)sizeof(E);
-
-// Sum over the TPR threads of a row; the same value in each of them.
+// Sums of two values over the TPR threads of a row, the same in each of them.
+// `turn` alternates between two places in LDS: one barrier a sum.
 template <int TPR>
-DEV_INLINE float row_sum(float v, float* lds) {
-    v = wave_sum(v);
+DEV_INLINE void row_sums(float& a, float& b, float2 (*lds)[16], int& turn) {
+    a = wave_sum(a);
+    b = wave_sum(b);
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
-        __syncthreads();  // the last sum's readers are done
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = make_float2(a, b);
         __syncthreads();
-        v = 0.0f;
+        a = b = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) v += lds[w];
+        for (int w = 0; w < W; ++w) {
+            a += lds[turn][w].x;
+            b += lds[turn][w].y;
+        }
+        turn ^= 1;
     }
-    return v;
 }
 
-// A row of `dim` elements over TPR threads, NV runs each: thread i holds the
-// runs i, i + TPR, ... The mean comes off before squaring: the variance of a
-// row far from zero does not cancel.
+// A thread's share of a row: run k starts at element at[k], and its elements
+// from skip[k] on are the thread's own. A row's last run starts early, so that
+// it is whole too; what it shares with the run before it is computed in both,
+// stored twice with one value, and summed in one. A run past the row is all
+// skipped. Needs dim >= RUN.
 template <typename E, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+struct Share {
+    int at[NV], skip[NV];
+    DEV_INLINE explicit Share(int dim) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = ((int)(threadIdx.x % TPR) + k * TPR) * RUN<E>;
+            at[k] = c < dim - RUN<E> ? c : dim - RUN<E>;
+            skip[k] = c - at[k];
+        }
+    }
+};
+
+// A run as it lies in memory.
+template <typename E>
+struct Raw {
+    E v[RUN<E>];
+    DEV_INLINE void load(const E* p) { load_run<E, RUN<E>>(p, RUN<E>, v); }
+    DEV_INLINE float operator[](int i) const { return to_f(v[i]); }
+};
+
+// Threads of a block: four rows of a wave each, or one row, whose waves meet at
+// barriers.
+constexpr int block_of(int tpr) { return tpr > 64 ? tpr : 256; }
+
+// Rows blockIdx, blockIdx + gridDim, ... of ROWS each, TPR threads and NV runs a
+// thread to a row. The weights stay in registers, and a row's loads go out
+// before the row in front of it is reduced. The mean comes off before squaring:
+// the variance of a row far from zero does not cancel.
+template <typename E, int TPR, int NV, bool FUSED>
+__global__ void __launch_bounds__(block_of(TPR))
 norm_fwd_kernel(const E* __restrict__ x, const E* __restrict__ res,
                 const E* __restrict__ w, const E* __restrict__ b,
                 E* __restrict__ y, E* __restrict__ s_out,
                 int64_t rows, int dim, float eps) {
-    constexpr int R = RUN<E>;
-    constexpr int ROWS = TPR > 256 ? 1 : 256 / TPR;
-    __shared__ float lds[16];
-    const int tid = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (row >= rows) return;  // TPR >= 256: a block is one row, none diverges
-    const E* xr = x + row * dim;
-    float v[NV][R];
-    float sum = 0.0f;
+    constexpr int R = RUN<E>, ROWS = block_of(TPR) / TPR;
+    __shared__ float2 lds[2][16];
+    const Share<E, TPR, NV> my(dim);
+    Raw<E> wr[NV], br[NV], xr[NV], rr[NV];
+    int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    const auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            xr[k].load(x + row * dim + my.at[k]);
+            if (FUSED) rr[k].load(res + row * dim + my.at[k]);
+        }
+    };
+    if (row < rows) fetch(row);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int c = (tid + k * TPR) * R, have = dim - c;
-        E in[R];
-        if (have > 0) {
-            load_run<E, R>(xr + c, have, in);
+        wr[k].load(w + my.at[k]);
+        if (b) br[k].load(b + my.at[k]);
+    }
+    int turn = 0;
+    // a block of one row at a time leaves the loop as one
+    for (; row < rows; row += (int64_t)gridDim.x * ROWS) {
+        float v[NV][R], sum = 0.0f, sq = 0.0f, none = 0.0f;
 #pragma unroll
-            for (int i = 0; i < R; ++i) v[k][i] = to_f(in[i]);
-            if (res) {
-                load_run<E, R>(res + row * dim + c, have, in);
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                v[k][i] = xr[k][i] + (FUSED ? rr[k][i] : 0.0f);
+                sum += i >= my.skip[k] ? v[k][i] : 0.0f;
+            }
+            if (FUSED && my.skip[k] < R) {
                 E so[R];
 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    v[k][i] += to_f(in[i]);
-                    so[i] = from_f<E>(v[k][i]);
-                }
-                store_run<E, R>(s_out + row * dim + c, have, so);
+                for (int i = 0; i < R; ++i) so[i] = from_f<E>(v[k][i]);
+                store_run<E, R>(s_out + row * dim + my.at[k], R, so);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < R; ++i) v[k][i] = 0.0f;
         }
+        const int64_t next = row + (int64_t)gridDim.x * ROWS;
+        if (next < rows) fetch(next);
+        row_sums<TPR>(sum, none, lds, turn);
+        const float mean = sum / dim;
 #pragma unroll
-        for (int i = 0; i < R; ++i) sum += v[k][i];
-    }
-    const float mean = row_sum<TPR>(sum, lds) / dim;
-    float sq = 0.0f;
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+            for (int i = 0; i < R; ++i) {
+                v[k][i] -= mean;
+                sq += i >= my.skip[k] ? v[k][i] * v[k][i] : 0.0f;
+            }
+        row_sums<TPR>(sq, none, lds, turn);
+        const float rstd = 1.0f / sqrtf(sq / dim + eps);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const float d = v[k][i] - mean;
-            if ((tid + k * TPR) * R + i < dim) sq += d * d;
+        for (int k = 0; k < NV; ++k) {
+            if (my.skip[k] >= R) continue;
+            E out[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                out[i] = from_f<E>(v[k][i] * rstd * wr[k][i] + (b ? br[k][i] : 0.0f));
+            store_run<E, R>(y + row * dim + my.at[k], R, out);
         }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, lds) / dim + eps);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (tid + k * TPR) * R, have = dim - c;
-        if (have <= 0) continue;
-        E win[R], bin[R], out[R];
-        load_run<E, R>(w + c, have, win);
-        if (b) load_run<E, R>(b + c, have, bin);
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-            out[i] = from_f<E>((v[k][i] - mean) * rstd * to_f(win[i]) +
-                               (b ? to_f(bin[i]) : 0.0f));
-        store_run<E, R>(y + row * dim + c, have, out);
     }
 }
 
-// Rows blockIdx, blockIdx + gridDim, ... of ROWS each; a thread's columns stay
-// the same from row to row, so the weight's gradient sums up in registers and
-// leaves once a block, as a row of part [gridDim][2][dim].
+// The same walk. A thread's columns stay the same from row to row, so the
+// weight's gradient sums up in registers and leaves once a block, as a row of
+// part [gridDim][2][dim].
 //
 // s is summed again from x and r, not read back as the forward pass rounded it:
 // in bf16 that rounding alone would add half again to the error of dw. The mean
 // and rstd come from the same registers. The sums join in two rounds: those of
 // s and g, then those of (s - mean)^2 and g (s - mean).
-template <typename E, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+template <typename E, int TPR, int NV, bool FUSED>
+__global__ void __launch_bounds__(block_of(TPR))
 norm_bwd_kernel(const E* __restrict__ x, const E* __restrict__ res,
                 const E* __restrict__ w, const E* __restrict__ dy,
                 const E* __restrict__ ds, E* __restrict__ dx,
                 float* __restrict__ part, int64_t rows, int dim, float eps) {
-    constexpr int R = RUN<E>;
-    constexpr int ROWS = TPR > 256 ? 1 : 256 / TPR;
-    __shared__ float lds[16];
-    const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    constexpr int R = RUN<E>, ROWS = block_of(TPR) / TPR;
+    __shared__ float2 lds[2][16];
+    const Share<E, TPR, NV> my(dim);
+    Raw<E> wr[NV], xr[NV], rr[NV], dr[NV], pr[NV];
     float dw[NV][R] = {}, db[NV][R] = {};
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < rows;
-         row += (int64_t)gridDim.x * ROWS) {
-        float n[NV][R], d[NV][R], g[NV][R];
-        float sum = 0.0f, sg = 0.0f;
+    const int sub = threadIdx.x / TPR, tid = threadIdx.x % TPR;
+    int64_t row = (int64_t)blockIdx.x * ROWS + sub;
+    const auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = (tid + k * TPR) * R, have = dim - c;
-            E xin[R], rin[R], din[R], win[R];
-            if (have > 0) {
-                load_run<E, R>(x + row * dim + c, have, xin);
-                if (res) load_run<E, R>(res + row * dim + c, have, rin);
-                load_run<E, R>(dy + row * dim + c, have, din);
-                load_run<E, R>(w + c, have, win);
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const bool real = i < have;
-                n[k][i] = real ? to_f(xin[i]) + (res ? to_f(rin[i]) : 0.0f) : 0.0f;
-                d[k][i] = real ? to_f(din[i]) : 0.0f;
-                g[k][i] = real ? d[k][i] * to_f(win[i]) : 0.0f;
-                sum += n[k][i];
-                sg += g[k][i];
-            }
+            xr[k].load(x + row * dim + my.at[k]);
+            if (FUSED) rr[k].load(res + row * dim + my.at[k]);
+            dr[k].load(dy + row * dim + my.at[k]);
         }
-        const float mean = row_sum<TPR>(sum, lds) / dim;
-        sg = row_sum<TPR>(sg, lds) / dim;
-        float sq = 0.0f, sgn = 0.0f;
+    };
+    if (row < rows) fetch(row);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) wr[k].load(w + my.at[k]);
+    int turn = 0;
+    for (; row < rows; row += (int64_t)gridDim.x * ROWS) {
+        float n[NV][R], d[NV][R], sum = 0.0f, sg = 0.0f, sq = 0.0f, sgn = 0.0f;
+        if (FUSED && ds)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) pr[k].load(ds + row * dim + my.at[k]);
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                n[k][i] = (tid + k * TPR) * R + i < dim ? n[k][i] - mean : 0.0f;
-                sq += n[k][i] * n[k][i];
-                sgn += g[k][i] * n[k][i];
+                n[k][i] = xr[k][i] + (FUSED ? rr[k][i] : 0.0f);
+                d[k][i] = dr[k][i];
+                const bool own = i >= my.skip[k];
+                sum += own ? n[k][i] : 0.0f;
+                sg += own ? d[k][i] * wr[k][i] : 0.0f;
+                db[k][i] += own ? d[k][i] : 0.0f;
             }
-        const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, lds) / dim + eps);
-        sgn = row_sum<TPR>(sgn, lds) * rstd / dim;
+        const int64_t next = row + (int64_t)gridDim.x * ROWS;
+        if (next < rows) fetch(next);
+        row_sums<TPR>(sum, sg, lds, turn);
+        const float mean = sum / dim;
+        sg /= dim;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (tid + k * TPR) * R, have = dim - c;
-            if (have <= 0) continue;
-            E out[R], pass[R];
-            if (ds) load_run<E, R>(ds + row * dim + c, have, pass);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                n[k][i] *= rstd;
-                dw[k][i] += d[k][i] * n[k][i];
-                db[k][i] += d[k][i];
-                out[i] = from_f<E>((g[k][i] - sg - n[k][i] * sgn) * rstd +
-                                   (ds ? to_f(pass[i]) : 0.0f));
+                const bool own = i >= my.skip[k];
+                n[k][i] -= mean;
+                sq += own ? n[k][i] * n[k][i] : 0.0f;
+                sgn += own ? d[k][i] * wr[k][i] * n[k][i] : 0.0f;
             }
-            store_run<E, R>(dx + row * dim + c, have, out);
+        row_sums<TPR>(sq, sgn, lds, turn);
+        const float rstd = 1.0f / sqrtf(sq / dim + eps);
+        sgn *= rstd / dim;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            E out[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const float m = n[k][i] * rstd;
+                dw[k][i] += i >= my.skip[k] ? d[k][i] * m : 0.0f;
+                out[i] = from_f<E>((d[k][i] * wr[k][i] - sg - m * sgn) * rstd +
+                                   (FUSED && ds ? pr[k][i] : 0.0f));
+            }
+            if (my.skip[k] < R) store_run<E, R>(dx + row * dim + my.at[k], R, out);
         }
     }
     // the block's ROWS rows of sums into one
@@ -177,7 +218,6 @@ norm_bwd_kernel(const E* __restrict__ x, const E* __restrict__ res,
     float* pw = part + (int64_t)blockIdx.x * 2 * dim;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int c = (tid + k * TPR) * R, have = dim - c;
         if constexpr (ROWS > 1) {
             __syncthreads();
 #pragma unroll
@@ -195,20 +235,25 @@ norm_bwd_kernel(const E* __restrict__ x, const E* __restrict__ res,
                     }
             }
         }
-        if (sub == 0 && have > 0) {
-            store_run<float, R>(pw + c, have, dw[k]);
-            store_run<float, R>(pw + dim + c, have, db[k]);
-        }
+        if (sub == 0)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i >= my.skip[k]) {
+                    pw[my.at[k] + i] = dw[k][i];
+                    pw[dim + my.at[k] + i] = db[k][i];
+                }
     }
 }
 
-// Rows too long for registers: the row is read again for each sum over it.
+// Rows shorter than a run or too long for registers: the row is read again for
+// each sum over it.
 template <typename E>
 __global__ void __launch_bounds__(1024)
 norm_fwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
                      const E* __restrict__ w, const E* __restrict__ b,
                      E* __restrict__ y, E* __restrict__ s_out, int dim, float eps) {
-    __shared__ float lds[16];
+    __shared__ float2 lds[2][16];
+    int turn = 0;
     const int64_t row = blockIdx.x;
     const E* xr = x + row * dim;
     const E* rr = res ? res + row * dim : nullptr;
@@ -218,13 +263,15 @@ norm_fwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
         if (rr) s_out[row * dim + c] = from_f<E>(v);
         sum += v;
     }
-    const float mean = row_sum<1024>(sum, lds) / dim;
-    float sq = 0.0f;
+    float sq = 0.0f, none = 0.0f;
+    row_sums<1024>(sum, none, lds, turn);
+    const float mean = sum / dim;
     for (int c = threadIdx.x; c < dim; c += 1024) {
         const float d = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean;
         sq += d * d;
     }
-    const float rstd = 1.0f / sqrtf(row_sum<1024>(sq, lds) / dim + eps);
+    row_sums<1024>(sq, none, lds, turn);
+    const float rstd = 1.0f / sqrtf(sq / dim + eps);
     for (int c = threadIdx.x; c < dim; c += 1024) {
         const float v = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
         y[row * dim + c] = from_f<E>((v - mean) * rstd * to_f(w[c]) +
@@ -239,7 +286,8 @@ __global__ void __launch_bounds__(1024)
 norm_bwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
                      const E* __restrict__ w, float* __restrict__ stats, const E* __restrict__ dy,
                      const E* __restrict__ ds, E* __restrict__ dx, int dim, float eps) {
-    __shared__ float lds[16];
+    __shared__ float2 lds[2][16];
+    int turn = 0;
     const int64_t row = blockIdx.x;
     const E *xr = x + row * dim, *rr = res ? res + row * dim : nullptr, *dr = dy + row * dim;
     float sum = 0.0f, sg = 0.0f, sq = 0.0f, sgn = 0.0f;
@@ -247,15 +295,17 @@ norm_bwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
         sum += to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
         sg += to_f(dr[c]) * to_f(w[c]);
     }
-    const float mean = row_sum<1024>(sum, lds) / dim;
-    sg = row_sum<1024>(sg, lds) / dim;
+    row_sums<1024>(sum, sg, lds, turn);
+    const float mean = sum / dim;
+    sg /= dim;
     for (int c = threadIdx.x; c < dim; c += 1024) {
         const float n = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean;
         sq += n * n;
         sgn += to_f(dr[c]) * to_f(w[c]) * n;
     }
-    const float rstd = 1.0f / sqrtf(row_sum<1024>(sq, lds) / dim + eps);
-    sgn = row_sum<1024>(sgn, lds) * rstd / dim;
+    row_sums<1024>(sq, sgn, lds, turn);
+    const float rstd = 1.0f / sqrtf(sq / dim + eps);
+    sgn *= rstd / dim;
     if (threadIdx.x == 0) {
         stats[2 * row] = mean;
         stats[2 * row + 1] = rstd;
@@ -286,30 +336,47 @@ norm_dw_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
     part[((int64_t)blockIdx.y * 2 + 1) * dim + c] = db;
 }
 
-// Runs of a row, and by them the smallest group of threads that holds it: a
-// wave up to 4 runs a lane, then 256 and 1024 threads. 0: too long.
+// By the runs of a row, the smallest group of threads that holds it with two
+// runs a thread: in bf16 more leave the registers of one wave a SIMD. 0 threads:
+// longer than 8192 elements, or shorter than a run.
 struct Shape {
     int threads, runs;
 };
 template <typename E>
 Shape shape_of(int dim) {
     const int runs = (dim + RUN<E> - 1) / RUN<E>;
-    for (int t : {64, 256, 1024})
-        for (int nv : {1, 2, 4})
-            if (runs <= t * nv) return {t, nv};
+    if (dim < RUN<E>) return {0, 0};
+    if (runs <= 64) return {64, 1};
+    for (int t : {64, 128, 256, 512})
+        if (runs <= t * 2) return {t, 2};
+    if (sizeof(E) == 4 && runs <= 512 * 4) return {512, 4};
     return {0, 0};
 }
 
 template <typename E, typename F>
-void with_shape(int dim, F&& f) {
+void with_shape(int dim, bool fused, F&& f) {
     const Shape p = shape_of<E>(dim);
-#define CASE(T, N) \
-    if (p.threads == T && p.runs == N) \
-    return f(std::integral_constant<int, T>(), std::integral_constant<int, N>())
-    CASE(64, 1); CASE(64, 2); CASE(64, 4);
-    CASE(256, 2); CASE(256, 4);
-    CASE(1024, 2); CASE(1024, 4);
-#undef CASE
+    const auto go = [&](auto t, auto n) {
+        if (p.threads != t || p.runs != n) return;
+        fused ? f(t, n, std::true_type()) : f(t, n, std::false_type());
+    };
+    go(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    go(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    go(std::integral_constant<int, 128>(), std::integral_constant<int, 2>());
+    go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+    go(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
+    if constexpr (sizeof(E) == 4)
+        go(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
+}
+
+// Blocks of a launch: enough to fill the card several times over, and few
+// enough that each keeps its weights for several rows.
+constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 512;
+
+int blocks_of(int64_t rows, int threads, int64_t most) {
+    const int each = block_of(threads) / threads;
+    const int64_t need = (rows + each - 1) / each;
+    return (int)(need < most ? need : most);
 }
 
 template <typename E>
@@ -321,11 +388,10 @@ int fwd(const void* x, const void* res, const void* w, const void* b, void* y,
             (const E*)x, (const E*)res, (const E*)w, (const E*)b, (E*)y, (E*)s,
             dim, eps);
     else
-        with_shape<E>(dim, [&](auto t, auto n) {
+        with_shape<E>(dim, res != nullptr, [&](auto t, auto n, auto fused) {
             constexpr int T = decltype(t)::value, N = decltype(n)::value;
-            constexpr int ROWS = T > 256 ? 1 : 256 / T;
-            norm_fwd_kernel<E, T, N>
-                <<<dim3((unsigned)((rows + ROWS - 1) / ROWS)), T > 256 ? T : 256, 0, st>>>(
+            norm_fwd_kernel<E, T, N, decltype(fused)::value>
+                <<<blocks_of(rows, T, FWD_BLOCKS), block_of(T), 0, st>>>(
                     (const E*)x, (const E*)res, (const E*)w, (const E*)b, (E*)y,
                     (E*)s, rows, dim, eps);
         });
@@ -346,17 +412,15 @@ int bwd(const void* x, const void* res, const void* w, const void* dy, const voi
         norm_dw_long_kernel<E><<<dim3((dim + 255) / 256, parts), 256, 0, st>>>(
             (const E*)x, (const E*)res, stats, (const E*)dy, part, rows, dim);
     } else {
-        with_shape<E>(dim, [&](auto t, auto n) {
+        with_shape<E>(dim, res != nullptr, [&](auto t, auto n, auto fused) {
             constexpr int T = decltype(t)::value, N = decltype(n)::value;
-            norm_bwd_kernel<E, T, N><<<parts, T > 256 ? T : 256, 0, st>>>(
+            norm_bwd_kernel<E, T, N, decltype(fused)::value><<<parts, block_of(T), 0, st>>>(
                 (const E*)x, (const E*)res, (const E*)w, (const E*)dy, (const E*)ds, (E*)dx, part,
                 rows, dim, eps);
         });
     }
     LSTM_CHECK_LAUNCH();
-    column_sum_kernel<E><<<(2 * dim + 63) / 64, 1024, 0, st>>>(part, (E*)dwb, parts, 2 * dim);
-    LSTM_CHECK_LAUNCH();
-    return 0;
+    return column_sum<E>(part, (E*)dwb, parts, 2 * dim, st);
 }
 
 }  // namespace
@@ -372,8 +436,7 @@ extern "C" int launch_norm_fwd(int is_bf16, const void* x, const void* res, cons
 // for each), and floats of `stats`, which only the rows past registers need.
 extern "C" int norm_bwd_parts(int is_bf16, int64_t rows, int dim) {
     const Shape p = is_bf16 ? shape_of<bf16>(dim) : shape_of<float>(dim);
-    const int64_t groups = p.threads == 64 ? (rows + 3) / 4 : rows;
-    return (int)(groups < 512 ? groups : 512);
+    return blocks_of(rows, p.threads ? p.threads : 1024, BWD_BLOCKS);
 }
 
 extern "C" int64_t norm_bwd_stats(int is_bf16, int64_t rows, int dim) {
