@@ -25,12 +25,12 @@ DEV_INLINE void sigmoid_pair(float x, float& pos, float& neg) {
     neg = x >= 0.0f ? small : big;
 }
 
-// silu(x) = x * sigma(x) and its derivative sigma + x sigma (1 - sigma).
+// silu(x) = x * sigma(x) and its derivative sigma + x sigma (1 - sigma). Where
+// sigma nears one, 1 - sigma is off by a rounding of one, as is what it is added to.
 DEV_INLINE void silu_grad(float x, float& val, float& grad) {
-    float s, n;
-    sigmoid_pair(x, s, n);
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
     val = x * s;
-    grad = s * (1.0f + x * n);
+    grad = s + val * (1.0f - s);
 }
 
 // N consecutive elements in one memory instruction, whatever their alignment
@@ -86,9 +86,9 @@ template <> struct Two<bf16> {
     }
 };
 
-// Sum over a wave, the same in each lane: four steps inside rows of 16 lanes as
-// operands of the additions, two across rows by lane swaps, none through LDS.
-DEV_INLINE float wave_sum(float v) {
+// Sum over a row of 16 lanes, the same in each: operands of the additions are
+// the other lanes' values, none goes through LDS.
+DEV_INLINE float row_sum16(float v) {
 #ifdef __HIP_DEVICE_COMPILE__
     const auto turned = [](float x, auto control) {
         return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x),
@@ -98,6 +98,14 @@ DEV_INLINE float wave_sum(float v) {
     v += turned(v, std::integral_constant<int, 0x4e>());   // lane ^ 2
     v += turned(v, std::integral_constant<int, 0x141>());  // half a row mirrored
     v += turned(v, std::integral_constant<int, 0x140>());  // a row mirrored
+#endif
+    return v;
+}
+
+// Sum over a wave, the same in each lane: across the rows by lane swaps.
+DEV_INLINE float wave_sum(float v) {
+    v = row_sum16(v);
+#ifdef __HIP_DEVICE_COMPILE__
     const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v),
                                                        false, false);
     v = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);

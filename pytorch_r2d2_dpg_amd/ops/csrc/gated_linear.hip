@@ -51,9 +51,12 @@ enum class Lie { K, INDEX };
 
 // One operand's tile of SPAN indexes by DEPTH k, in LDS as the operand lies in
 // memory, its pieces permuted so that the lanes that read together meet
-// different banks: by the row's low bits where k lies together, by pairs of
-// pieces and k's low two bits for the transposing reads.
-template <typename E, Lie LIE, int SPAN, int THREADS, bool DIRECT>
+// different banks: by the low bits of the row's place in its fragment where k
+// lies together, by pairs of pieces and k's low two bits for the transposing reads.
+// JUMP: a fragment's 16 indexes are four runs of 4, 4 * JUMP apart; JUMP of
+// them, 4 apart, cover 16 * JUMP indexes, and a lane's accumulators 4 * JUMP
+// neighbours of the result, which it stores in one piece.
+template <typename E, Lie LIE, int SPAN, int THREADS, bool DIRECT, int JUMP>
 struct Operand {
     static constexpr int P = PIECE<E>, PIECES = SPAN * 8, ROUNDS = PIECES / THREADS;
     static constexpr int ROW = LIE == Lie::K ? 8 : SPAN / P;  // pieces of a row in LDS
@@ -64,7 +67,7 @@ struct Operand {
     u4 held[DIRECT ? 1 : ROUNDS];
 
     static DEV_INLINE int swizzle(int row, int piece) {
-        return LIE == Lie::K ? piece ^ (row & 7)
+        return LIE == Lie::K ? piece ^ ((row & 3) | (row / (4 * JUMP) & 1) << 2)
                              : sizeof(E) == 2 ? piece ^ ((row & 3) << 1) : piece;
     }
 
@@ -122,12 +125,12 @@ struct Operand {
             for (int r = 0; r < ROUNDS; ++r) tile[r * THREADS + threadIdx.x] = held[r];
     }
 
-    // The piece of the matrix instructions for the 16 indexes from `first`, at
-    // the tile's k from `k` pieces of four groups on.
+    // The piece of the matrix instructions for the 16 indexes of the fragment that
+    // starts at `first`, at the tile's k from `k` pieces of four groups on.
     static DEV_INLINE u4 read(const u4* tile, int first, int k) {
         const int lane = threadIdx.x & 63, group = lane >> 4;
         if constexpr (LIE == Lie::K) {
-            const int row = first + (lane & 15);
+            const int row = first + (lane >> 2 & 3) * 4 * JUMP + (lane & 3);
             return tile[row * 8 + swizzle(row, k * 4 + group)];
         } else if constexpr (sizeof(E) == 2) {
             // 16 lanes read 4 k by 16 indexes, 8 bytes each, and get back the 4 k
@@ -192,6 +195,138 @@ struct Tile {
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
 };
 
+template <typename E, int N, bool INSIDE>
+DEV_INLINE void load_piece(const E* p, int have, E (&v)[N]) {
+    if constexpr (INSIDE) have = N;
+    load_run<E, N>(p, have, v);
+}
+template <typename E, int N, bool INSIDE>
+DEV_INLINE void store_piece(E* p, int have, const E (&v)[N]) {
+    if constexpr (INSIDE) have = N;
+    store_run<E, N>(p, have, v);
+}
+
+template <typename E, typename T, End END, bool INSIDE>
+DEV_INLINE void finish(const Args<E>& p, const f4 (&acc)[T::MI][T::NI], int tm, int m0, int n0,
+                       void* lds) {
+    constexpr bool GATED = END == End::GATED || END == End::GATED_GRAD;
+    constexpr int HALF = T::BN / 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / T::WN, wn = wave % T::WN;
+    const int row0 = m0 + wm * T::MI * 16 + (lane & 15);
+    if constexpr (GATED) {
+        constexpr int NB = T::NI / 2, C = 4 * NB;
+        const int in = wn * NB * 16 + (lane >> 4) * C, col = n0 + in, have = p.N - col;
+        float bg[C] = {}, bu[C] = {}, sg[C] = {}, su[C] = {};
+        if (p.bias) {
+            E g[C], u[C];
+            load_piece<E, C, INSIDE>(p.bias + col, have, g);
+            load_piece<E, C, INSIDE>(p.bias + p.N + col, have, u);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                bg[c] = to_f(g[c]);
+                bu[c] = to_f(u[c]);
+            }
+        }
+        E d[C];
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i) {
+            const int row = row0 + i * 16;
+            if (!INSIDE && (row >= p.M || have <= 0)) continue;
+            if (END == End::GATED_GRAD)
+                load_piece<E, C, INSIDE>(p.dy + (int64_t)row * p.N + col, have, d);
+            E out[C], out2[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float g = acc[i][c / 4][c % 4] + bg[c];
+                const float u = acc[i][c / 4 + NB][c % 4] + bu[c];
+                float val, grad;
+                silu_grad(g, val, grad);
+                if (END == End::GATED) {
+                    out[c] = from_f<E>(val * u);
+                } else {
+                    const float dg = to_f(d[c]) * u * grad, du = to_f(d[c]) * val;
+                    out[c] = from_f<E>(dg);
+                    out2[c] = from_f<E>(du);
+                    sg[c] += dg;
+                    su[c] += du;
+                }
+            }
+            if (END == End::GATED) {
+                store_piece<E, C, INSIDE>(p.out + (int64_t)row * p.N + col, have, out);
+            } else {
+                E* to = p.out + (int64_t)row * 2 * p.N + col;
+                store_piece<E, C, INSIDE>(to, have, out);
+                store_piece<E, C, INSIDE>(to + p.N, have, out2);
+            }
+        }
+        if (END == End::GATED_GRAD && p.part) {
+            float* sums = reinterpret_cast<float*>(lds);  // [WM][2][HALF]
+            __syncthreads();  // the tiles in LDS have been read
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float a = row_sum16(sg[c]), b = row_sum16(su[c]);
+                if ((lane & 15) == 0) {
+                    sums[(wm * 2) * HALF + in + c] = a;
+                    sums[(wm * 2 + 1) * HALF + in + c] = b;
+                }
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < 2 * HALF; c += T::THREADS) {
+                const int which = c / HALF, at = c % HALF;
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < T::WM; ++w) s += sums[(w * 2 + which) * HALF + at];
+                if (n0 + at < p.N)
+                    p.part[(int64_t)tm * 2 * p.N + which * (int64_t)p.N + n0 + at] = s;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i) {
+            const int row = row0 + i * 16;
+            if (!INSIDE && row >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < T::NI; ++j) {
+                const int col = n0 + (wn * T::NI + j) * 16 + (lane >> 4) * 4, have = p.N - col;
+                if (!INSIDE && have <= 0) continue;
+                const int64_t at = (int64_t)row * p.N + col;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                if (END == End::PLAIN) {
+                    E out[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) out[q] = from_f<E>(v[q]);
+                    store_piece<E, 4, INSIDE>(p.out + at, have, out);
+                } else {
+                    store_piece<float, 4, INSIDE>(
+                        p.part + blockIdx.z * (int64_t)p.M * p.N + at, have, v);
+                }
+            }
+        }
+    }
+}
+
+// The order of a tile's instructions: the first half's fragments are read, then
+// the second half's between the first half's products.
+template <typename E, Lie LA, Lie LB, typename T>
+DEV_INLINE void interleave() {
+#ifdef __HIP_DEVICE_COMPILE__
+    // LDS instructions a fragment, products a fragment pair
+    constexpr int RA = LA == Lie::K ? 1 : sizeof(E) == 2 ? 2 : 4;
+    constexpr int RB = LB == Lie::K ? 1 : sizeof(E) == 2 ? 2 : 4;
+    constexpr int READS = T::MI * RA + T::NI * RB;
+    constexpr int PRODUCTS = T::MI * T::NI * (sizeof(E) == 2 ? 1 : 4);
+    constexpr int EACH = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+    for (int r = 0; r < READS; ++r) {
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2 * PRODUCTS - EACH * READS, 0);
+#endif
+}
+
 template <typename E, typename T, Lie LA, Lie LB, End END, bool DIRECT>
 __global__ void __launch_bounds__(T::THREADS)
 product_kernel(Args<E> p) {
@@ -207,8 +342,9 @@ product_kernel(Args<E> p) {
     const int k_lo = blockIdx.z * p.per_split;
     const int k_hi = k_lo + p.per_split < p.K ? k_lo + p.per_split : p.K;
 
-    Operand<E, LA, T::BM, T::THREADS, DIRECT> a;
-    Operand<E, LB, T::BN, T::THREADS, DIRECT> b;
+    constexpr int NB = GATED ? T::NI / 2 : T::NI;  // a wave's fragments side by side
+    Operand<E, LA, T::BM, T::THREADS, DIRECT, 1> a;
+    Operand<E, LB, T::BN, T::THREADS, DIRECT, GATED ? NB : 1> b;
     a.start(p.a, p.pitch_a, p.M, [&](int i) {
         const int m = m0 + i;  // rows past the end read the last one: none is stored
         return (int64_t)(LA == Lie::K && m >= p.M ? p.M - 1 : m);
@@ -238,24 +374,26 @@ product_kernel(Args<E> p) {
             a.fetch(next, p.pitch_a, k0 + BD, k_hi);
             b.fetch(next + T::BM * 8, p.pitch_b, k0 + BD, k_hi);
         }
+        u4 af[2][T::MI], bf[2][T::NI];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            u4 af[T::MI], bf[T::NI];
 #pragma unroll
             for (int j = 0; j < T::NI; ++j) {
                 // gated: the wave's first half of columns are gates, then their values
-                constexpr int NH = T::NI / 2;
-                const int first = GATED ? (j / NH) * HALF + (wn * NH + j % NH) * 16
-                                        : (wn * T::NI + j) * 16;
-                bf[j] = b.read(now + T::BM * 8, first, k);
+                const int first = GATED ? (j / NB) * HALF + wn * NB * 16 + j % NB * 4
+                                        : (wn * NB + j) * 16;
+                bf[k][j] = b.read(now + T::BM * 8, first, k);
             }
 #pragma unroll
-            for (int i = 0; i < T::MI; ++i) af[i] = a.read(now, (wm * T::MI + i) * 16, k);
+            for (int i = 0; i < T::MI; ++i) af[k][i] = a.read(now, (wm * T::MI + i) * 16, k);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-                for (int j = 0; j < T::NI; ++j) acc[i][j] = mul(E(), bf[j], af[i], acc[i][j]);
-        }
+                for (int j = 0; j < T::NI; ++j) acc[i][j] = mul(E(), bf[k][j], af[k][i], acc[i][j]);
+        interleave<E, LA, LB, T>();
         if (more) {
             a.settle(next);
             b.settle(next + T::BM * 8);
@@ -263,100 +401,13 @@ product_kernel(Args<E> p) {
         turn ^= 1;
     }
 
-    // an accumulator's element q: row lane % 16, column (lane / 16) * 4 + q
-    const int row0 = m0 + wm * T::MI * 16 + (lane & 15);
-    if constexpr (GATED) {
-        constexpr int NH = T::NI / 2;
-        float* sums = reinterpret_cast<float*>(lds);  // [WM][2][HALF]
-        if (END == End::GATED_GRAD && p.part) __syncthreads();
-#pragma unroll
-        for (int j = 0; j < NH; ++j) {
-            const int in = (wn * NH + j) * 16 + (lane >> 4) * 4, col = n0 + in, have = p.N - col;
-            E bg[4], bu[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) bg[q] = bu[q] = from_f<E>(0.0f);
-            if (p.bias && have > 0) {
-                load_run<E, 4>(p.bias + col, have, bg);
-                load_run<E, 4>(p.bias + p.N + col, have, bu);
-            }
-            float sg[4] = {}, su[4] = {};
-#pragma unroll
-            for (int i = 0; i < T::MI; ++i) {
-                const int row = row0 + i * 16;
-                if (row >= p.M || have <= 0) continue;
-                E out[4], out2[4], d[4];
-                if (END == End::GATED_GRAD) load_run<E, 4>(p.dy + (int64_t)row * p.N + col, have, d);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float g = acc[i][j][q] + to_f(bg[q]);
-                    const float u = acc[i][j + NH][q] + to_f(bu[q]);
-                    float val, grad;
-                    silu_grad(g, val, grad);
-                    if (END == End::GATED) {
-                        out[q] = from_f<E>(val * u);
-                    } else {
-                        const float dg = to_f(d[q]) * u * grad, du = to_f(d[q]) * val;
-                        out[q] = from_f<E>(dg);
-                        out2[q] = from_f<E>(du);
-                        sg[q] += dg;
-                        su[q] += du;
-                    }
-                }
-                if (END == End::GATED) {
-                    store_run<E, 4>(p.out + (int64_t)row * p.N + col, have, out);
-                } else {
-                    E* to = p.out + (int64_t)row * 2 * p.N + col;
-                    store_run<E, 4>(to, have, out);
-                    store_run<E, 4>(to + p.N, have, out2);
-                }
-            }
-            if (END == End::GATED_GRAD && p.part)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-#pragma unroll
-                    for (int s = 1; s < 16; s <<= 1) {
-                        sg[q] += __shfl_xor(sg[q], s, 64);
-                        su[q] += __shfl_xor(su[q], s, 64);
-                    }
-                    if ((lane & 15) == 0) {
-                        sums[(wm * 2) * HALF + in + q] = sg[q];
-                        sums[(wm * 2 + 1) * HALF + in + q] = su[q];
-                    }
-                }
-        }
-        if (END == End::GATED_GRAD && p.part) {
-            __syncthreads();
-            for (int c = threadIdx.x; c < 2 * HALF; c += T::THREADS) {
-                const int which = c / HALF, in = c % HALF;
-                float s = 0.0f;
-#pragma unroll
-                for (int w = 0; w < T::WM; ++w) s += sums[(w * 2 + which) * HALF + in];
-                if (n0 + in < p.N)
-                    p.part[(int64_t)tm * 2 * p.N + which * (int64_t)p.N + n0 + in] = s;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < T::MI; ++i) {
-            const int row = row0 + i * 16;
-            if (row >= p.M) continue;
-#pragma unroll
-            for (int j = 0; j < T::NI; ++j) {
-                const int col = n0 + (wn * T::NI + j) * 16 + (lane >> 4) * 4, have = p.N - col;
-                if (have <= 0) continue;
-                const int64_t at = (int64_t)row * p.N + col;
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                if (END == End::PLAIN) {
-                    E out[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) out[q] = from_f<E>(v[q]);
-                    store_run<E, 4>(p.out + at, have, out);
-                } else {
-                    store_run<float, 4>(p.part + blockIdx.z * (int64_t)p.M * p.N + at, have, v);
-                }
-            }
-        }
-    }
+    // Fragment j's accumulator holds row lane % 16 and, as its element q, column
+    // (lane / 16) * 4 * JUMP + 4 j + q. Tiles inside the result are stored
+    // without looking at each piece.
+    if (m0 + T::BM <= p.M && n0 + COLS <= p.N)
+        finish<E, T, END, true>(p, acc, tm, m0, n0, lds);
+    else
+        finish<E, T, END, false>(p, acc, tm, m0, n0, lds);
 }
 
 // out = sum over the splits of part, in their order.
