@@ -32,11 +32,11 @@ extern "C" int launch_recurrence_bwd(int, const void*, const float*, const int*,
                                      hipStream_t);
 extern "C" int launch_gated_linear_fwd(int, const void*, const void*, const void*, void*, int,
                                        int, int, hipStream_t);
-extern "C" int gated_linear_bias_parts(int, int, int);
-extern "C" int gated_linear_splits(int, int, int, int);
+extern "C" int gated_linear_bias_parts(int, int, int, int);
+extern "C" int64_t gated_linear_split_sums(int, int, int, int, int, int);
 extern "C" int launch_gated_linear_bwd(int, const void*, const void*, const void*, const void*,
                                        void*, void*, void*, void*, float*, float*, int, int, int,
-                                       int, hipStream_t);
+                                       hipStream_t);
 
 namespace {
 
@@ -175,10 +175,10 @@ LinearSizes check_linear(const Tensor& x, const Tensor& weight, const OptTensor&
     if (bias) check(*bias, "bias", x, x.scalar_type(), {2 * F});
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
-    // tiles of 128 by 64 at the least lie on one grid axis
-    TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST && (M / 128 + 1) * (F / 64 + 1) <= MOST &&
-                    (M / 128 + 1) * (K / 64 + 1) <= MOST && (F / 64 + 1) * (K / 64 + 1) <= MOST,
-                "x or weight is too large");
+    // tiles of 64 by 64 at the least lie on one grid axis
+    const int64_t m = M / 64 + 1, k = K / 64 + 1, f = 2 * F / 64 + 1;
+    TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST / 2 && m * f <= MOST && m * k <= MOST &&
+                    k * f <= MOST, "x or weight is too large");
     return {M, K, F};
 }
 
@@ -204,23 +204,20 @@ std::tuple<Tensor, Tensor, Tensor> gated_linear_bwd(Tensor x, Tensor weight, Opt
     check(dy, "dy", x, x.scalar_type(), shape);
     const auto f32 = x.options().dtype(torch::kFloat32);
     auto dp = torch::empty({n.M, 2 * n.F}, x.options());
-    Tensor dx, dw, db, part_db, part_dw;
-    const int splits = gated_linear_splits(is_bf16(x), (int)n.M, (int)n.K, (int)n.F);
+    Tensor dx, dw, db, part_db;
+    const int M = (int)n.M, K = (int)n.K, F = (int)n.F, half = is_bf16(x);
     if (need_x) dx = torch::empty_like(x);
-    if (need_w) {
-        dw = torch::empty_like(weight);
-        part_dw = torch::empty({splits > 1 ? splits : 0, 2 * n.F, n.K}, f32);
-    }
+    if (need_w) dw = torch::empty_like(weight);
     if (need_b) {
         db = torch::empty({2 * n.F}, x.options());
-        part_db = torch::empty({gated_linear_bias_parts(is_bf16(x), (int)n.M, (int)n.F), 2 * n.F}, f32);
+        part_db = torch::empty({gated_linear_bias_parts(half, M, K, F), 2 * n.F}, f32);
     }
+    auto part = torch::empty({gated_linear_split_sums(half, M, K, F, need_x, need_w)}, f32);
     const int rc = launch_gated_linear_bwd(
-        is_bf16(x), x.data_ptr(), weight.data_ptr(), ptr(bias), dy.data_ptr(), dp.data_ptr(),
+        half, x.data_ptr(), weight.data_ptr(), ptr(bias), dy.data_ptr(), dp.data_ptr(),
         need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
         need_b ? db.data_ptr() : nullptr, need_b ? part_db.data_ptr<float>() : nullptr,
-        need_w ? part_dw.data_ptr<float>() : nullptr, (int)n.M, (int)n.K, (int)n.F, splits,
-        stream());
+        part.data_ptr<float>(), M, K, F, stream());
     TORCH_CHECK(rc == 0, "gated linear backward launch failed");
     return {dx, dw, db};
 }

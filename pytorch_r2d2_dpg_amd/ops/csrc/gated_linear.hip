@@ -73,9 +73,11 @@ enum class Lie { K, INDEX };
 // neighbours of the result, which it stores in one piece.
 template <typename E, Lie LIE, int SPAN, int THREADS, bool DIRECT, int JUMP>
 struct Operand {
-    static constexpr int P = PIECE<E>, PIECES = SPAN * 8, ROUNDS = PIECES / THREADS;
+    static constexpr int P = PIECE<E>, PIECES = SPAN * 8;
+    static constexpr int ROUNDS = (PIECES + THREADS - 1) / THREADS;
     static constexpr int ROW = LIE == Lie::K ? 8 : SPAN / P;  // pieces of a row in LDS
-    static_assert(PIECES % THREADS == 0, "every thread stages as many pieces");
+    static constexpr int KEPT = (ROW & -ROW) - 1;  // bits that may turn without leaving it
+    static_assert(PIECES % 64 == 0, "a wave stages in a round or does not");
 
     const E* at[ROUNDS];  // this thread's pieces of the tile at k = 0
     int have[ROUNDS];     // elements of it along the index (INDEX), 0 or less: none
@@ -83,8 +85,14 @@ struct Operand {
 
     static DEV_INLINE int swizzle(int row, int piece) {
         return LIE == Lie::K    ? piece ^ ((row & 3) | (row / (4 * JUMP) & 1) << 2)
-               : sizeof(E) == 2 ? piece ^ ((row & 3) | (row >> 1 & 4)) << 1
-                                : piece ^ (row >> 2 & 3) << 2;
+               : sizeof(E) == 2 ? piece ^ (((row & 3) | (row >> 1 & 4)) << 1 & KEPT)
+                                : piece ^ ((row >> 2 & 3) << 2 & KEPT);
+    }
+
+    // Whether this wave has pieces in a round; in all but the last every one has.
+    static DEV_INLINE bool stages(int r) {
+        return (r + 1) * THREADS <= PIECES ||
+               r * THREADS + (int)__builtin_amdgcn_readfirstlane(threadIdx.x) < PIECES;
     }
 
     // `index(i)`: the operand's index for the tile's i-th, inside of it always
@@ -117,6 +125,7 @@ struct Operand {
         const bool whole = k0 + DEPTH<E> <= k_hi;
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
+            if (!stages(r)) continue;
             const E* p = at[r] + step;
             if constexpr (DIRECT) {
                 // aligned pitches: a piece exists whole or not at all
@@ -136,7 +145,8 @@ struct Operand {
     DEV_INLINE void settle(u4* tile) const {
         if constexpr (!DIRECT)
 #pragma unroll
-            for (int r = 0; r < ROUNDS; ++r) tile[r * THREADS + threadIdx.x] = held[r];
+            for (int r = 0; r < ROUNDS; ++r)
+                if (stages(r)) tile[r * THREADS + threadIdx.x] = held[r];
     }
 
     // The piece of the matrix instructions for the 16 indexes of the fragment that
@@ -208,6 +218,7 @@ template <int BM_, int BN_, int WM_, int WN_>
 struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+    static_assert(MI * WM * 16 == BM && NI * WN * 16 == BN, "whole fragments");
 };
 
 template <typename E, int N, bool INSIDE>
@@ -446,14 +457,54 @@ join_splits_kernel(const float* __restrict__ part, E* __restrict__ out, int64_t 
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-using Large = Tile<256, 256, 2, 4>;
-using Small = Tile<128, 128, 2, 2>;
+// The tiles that a product may be cut into, and what a CU reaches with each in
+// a long product (TFLOP/s), measured.
+template <typename E, typename F>
+void each_tile(F&& f) {
+    if constexpr (sizeof(E) == 2) {
+        f(Tile<256, 256, 2, 4>(), 4.9);
+        f(Tile<192, 256, 2, 4>(), 4.7);
+        f(Tile<160, 256, 2, 4>(), 4.5);
+        f(Tile<128, 256, 2, 4>(), 4.3);
+        f(Tile<128, 128, 2, 2>(), 3.4);
+        f(Tile<64, 64, 2, 2>(), 1.8);
+    } else {
+        f(Tile<128, 128, 2, 2>(), 0.5);
+        f(Tile<64, 64, 2, 2>(), 0.4);
+    }
+}
 
-// A tile of 256 x 256 reads half of what four of 128 x 128 do from L2 and LDS,
-// but a card of 256 CUs needs enough of them.
+// How a product is cut: which tile, and into how many splits of k, whose sums
+// join_splits_kernel adds.
+struct Cut {
+    int bm, bn, splits;
+};
+
+// The cut with the least estimated time: rounds of one tile a CU, each as long
+// as its k takes plus a tile's start and end, plus the splits' way through
+// memory. `wide` is N, or 2F where gate and value columns share a tile.
 template <typename E>
-bool large(int64_t m, int64_t n, int splits) {
-    return sizeof(E) == 2 && (int64_t)ceil_div(m, 256) * ceil_div(n, 256) * splits >= 256;
+Cut cut_of(int64_t m, int64_t wide, int64_t k, bool may_split) {
+    constexpr int64_t CUS = 256;
+    Cut best{0, 0, 1};
+    double least = 0;
+    each_tile<E>([&](auto tile, double rate) {
+        using T = decltype(tile);
+        const int64_t tiles = (int64_t)ceil_div(m, T::BM) * ceil_div(wide, T::BN);
+        const int64_t steps = ceil_div(k, DEPTH<E>);
+        for (int64_t splits = 1; splits <= 64; splits *= 2) {
+            if (splits > 1 && (!may_split || steps < 2 * splits)) break;
+            const int64_t rounds = (tiles * splits + CUS - 1) / CUS;
+            const double step = 2.0 * T::BM * T::BN * DEPTH<E> / rate * 1e-6;  // us
+            double us = rounds * (ceil_div(steps, splits) * step + 1.5 + T::BM * T::BN / 32768.0);
+            if (splits > 1) us += 3.0 + splits * m * wide * 8 / 4e6;
+            if (best.bm == 0 || us < least) {
+                least = us;
+                best = {T::BM, T::BN, (int)splits};
+            }
+        }
+    });
+    return best;
 }
 
 template <typename E, typename T, Lie LA, Lie LB, End END>
@@ -461,6 +512,7 @@ int launch(Args<E> p, int splits, hipStream_t st) {
     constexpr bool GATED = END == End::GATED || END == End::GATED_GRAD;
     p.tiles_m = ceil_div(p.M, T::BM);
     p.tiles_n = ceil_div(p.N, GATED ? T::BN / 2 : T::BN);
+    p.per_split = ceil_div(ceil_div(p.K > 0 ? p.K : 1, splits), DEPTH<E>) * DEPTH<E>;
     const dim3 grid(p.tiles_m * p.tiles_n, 1, splits);
     const auto whole = [](const void* q, int64_t pitch) {
         return (uintptr_t)q % 16 == 0 && pitch % PIECE<E> == 0;
@@ -474,12 +526,36 @@ int launch(Args<E> p, int splits, hipStream_t st) {
 }
 
 template <typename E, Lie LA, Lie LB, End END>
-int product(const Args<E>& p, int splits, hipStream_t st) {
-    constexpr bool GATED = END == End::GATED || END == End::GATED_GRAD;
-    if constexpr (sizeof(E) == 2)
-        if (large<E>(p.M, GATED ? 2 * (int64_t)p.N : p.N, splits))
-            return launch<E, Large, LA, LB, END>(p, splits, st);
-    return launch<E, Small, LA, LB, END>(p, splits, st);
+int product(const Args<E>& p, Cut cut, hipStream_t st) {
+    int rc = -1;
+    each_tile<E>([&](auto tile, double) {
+        using T = decltype(tile);
+        if (T::BM == cut.bm && T::BN == cut.bn) rc = launch<E, T, LA, LB, END>(p, cut.splits, st);
+    });
+    return rc;
+}
+
+// A plain product, in one piece or in splits through `part`.
+template <typename E, Lie LA, Lie LB>
+int plain(Args<E> p, Cut cut, float* part, hipStream_t st) {
+    if (cut.splits == 1) return product<E, LA, LB, End::PLAIN>(p, cut, st);
+    p.part = part;
+    const int rc = product<E, LA, LB, End::PART>(p, cut, st);
+    if (rc) return rc;
+    const int64_t n = (int64_t)p.M * p.N;
+    join_splits_kernel<E><<<ceil_div(n, 1024), 256, 0, st>>>(part, p.out, n, cut.splits);
+    LSTM_CHECK_LAUNCH();
+    return 0;
+}
+
+template <typename E> Cut cut_gated(int M, int K, int F) {
+    return cut_of<E>(M, 2 * (int64_t)F, K, false);
+}
+template <typename E> Cut cut_dx(int M, int K, int F) {
+    return cut_of<E>(M, K, 2 * (int64_t)F, true);
+}
+template <typename E> Cut cut_dw(int M, int K, int F) {
+    return cut_of<E>(2 * (int64_t)F, K, M, true);
 }
 
 template <typename E>
@@ -489,51 +565,50 @@ int fwd(const void* x, const void* w, const void* bias, void* y, int M, int K, i
     Args<E> p{};
     p.a = (const E*)x; p.pitch_a = K;
     p.b = (const E*)w; p.pitch_b = K;
-    p.M = M; p.N = F; p.K = K; p.per_split = K;
+    p.M = M; p.N = F; p.K = K;
     p.bias = (const E*)bias; p.out = (E*)y;
-    return product<E, Lie::K, Lie::K, End::GATED>(p, 1, st);
+    return product<E, Lie::K, Lie::K, End::GATED>(p, cut_gated<E>(M, K, F), st);
 }
 
+// Rows of 2F partial sums for db.
 template <typename E>
-int bias_parts(int M, int F) {
-    return ceil_div(M, large<E>(M, 2 * (int64_t)F, 1) ? Large::BM : Small::BM);
+int bias_parts(int M, int K, int F) {
+    return ceil_div(M, cut_gated<E>(M, K, F).bm);
 }
 
-// dw's products run along M, long where its tiles are few: splits of it fill the
-// card, each no shorter than 8 tiles deep.
+// Floats of partial sums for the splits of dx and dw, which take turns with them.
 template <typename E>
-int splits_of(int M, int K, int F) {
-    const int64_t tiles = (int64_t)ceil_div(2 * (int64_t)F, 128) * ceil_div(K, 128);
-    const int64_t want = ceil_div(512, tiles > 0 ? tiles : 1), most = M / (8 * DEPTH<E>);
-    const int64_t n = want < most ? want : most;
-    return (int)(n > 0 ? n : 1);
+int64_t split_sums(int M, int K, int F, bool dx, bool dw) {
+    const int sx = cut_dx<E>(M, K, F).splits, sw = cut_dw<E>(M, K, F).splits;
+    const int64_t nx = dx && sx > 1 ? (int64_t)sx * M * K : 0;
+    const int64_t nw = dw && sw > 1 ? (int64_t)sw * 2 * F * K : 0;
+    return nx > nw ? nx : nw;
 }
 
 template <typename E>
 int bwd(const void* x, const void* w, const void* bias, const void* dy, void* dp, void* dx,
-        void* dw, void* db, float* part_db, float* part_dw, int M, int K, int F, int splits,
-        hipStream_t st) {
+        void* dw, void* db, float* part_db, float* part, int M, int K, int F, hipStream_t st) {
     int rc = 0;
     if ((int64_t)M * F != 0) {
         Args<E> p{};
         p.a = (const E*)x; p.pitch_a = K;
         p.b = (const E*)w; p.pitch_b = K;
-        p.M = M; p.N = F; p.K = K; p.per_split = K;
+        p.M = M; p.N = F; p.K = K;
         p.bias = (const E*)bias; p.dy = (const E*)dy; p.out = (E*)dp; p.part = db ? part_db : nullptr;
-        rc = product<E, Lie::K, Lie::K, End::GATED_GRAD>(p, 1, st);
+        rc = product<E, Lie::K, Lie::K, End::GATED_GRAD>(p, cut_gated<E>(M, K, F), st);
         if (rc) return rc;
     }
     if (db && F) {
-        rc = column_sum<E>(part_db, (E*)db, bias_parts<E>(M, F), 2 * F, st);
+        rc = column_sum<E>(part_db, (E*)db, bias_parts<E>(M, K, F), 2 * F, st);
         if (rc) return rc;
     }
     if (dx && (int64_t)M * K != 0) {
         Args<E> p{};
         p.a = (const E*)dp; p.pitch_a = 2 * (int64_t)F;
         p.b = (const E*)w; p.pitch_b = K;
-        p.M = M; p.N = K; p.K = 2 * F; p.per_split = 2 * F;
+        p.M = M; p.N = K; p.K = 2 * F;
         p.out = (E*)dx;
-        rc = product<E, Lie::K, Lie::INDEX, End::PLAIN>(p, 1, st);
+        rc = plain<E, Lie::K, Lie::INDEX>(p, cut_dx<E>(M, K, F), part, st);
         if (rc) return rc;
     }
     if (dw && (int64_t)F * K != 0) {
@@ -541,14 +616,9 @@ int bwd(const void* x, const void* w, const void* bias, const void* dy, void* dp
         p.a = (const E*)dp; p.pitch_a = 2 * (int64_t)F;
         p.b = (const E*)x; p.pitch_b = K;
         p.M = 2 * F; p.N = K; p.K = M;
-        p.per_split = ceil_div(ceil_div(M > 0 ? M : 1, splits), DEPTH<E>) * DEPTH<E>;
-        p.part = part_dw; p.out = (E*)dw;
-        if (splits == 1) return product<E, Lie::INDEX, Lie::INDEX, End::PLAIN>(p, 1, st);
-        rc = product<E, Lie::INDEX, Lie::INDEX, End::PART>(p, splits, st);
+        p.out = (E*)dw;
+        rc = plain<E, Lie::INDEX, Lie::INDEX>(p, cut_dw<E>(M, K, F), part, st);
         if (rc) return rc;
-        const int64_t n = (int64_t)2 * F * K;
-        join_splits_kernel<E><<<ceil_div(n, 1024), 256, 0, st>>>(part_dw, (E*)dw, n, splits);
-        LSTM_CHECK_LAUNCH();
     }
     return 0;
 }
@@ -562,19 +632,17 @@ extern "C" int launch_gated_linear_fwd(int is_bf16, const void* x, const void* w
                    : fwd<float>(x, w, bias, y, M, K, F, st);
 }
 
-// Rows of 2F partial sums for db, and splits of 2F * K partial sums for dw (one:
-// none are needed).
-extern "C" int gated_linear_bias_parts(int is_bf16, int M, int F) {
-    return is_bf16 ? bias_parts<bf16>(M, F) : bias_parts<float>(M, F);
+extern "C" int gated_linear_bias_parts(int is_bf16, int M, int K, int F) {
+    return is_bf16 ? bias_parts<bf16>(M, K, F) : bias_parts<float>(M, K, F);
 }
-extern "C" int gated_linear_splits(int is_bf16, int M, int K, int F) {
-    return is_bf16 ? splits_of<bf16>(M, K, F) : splits_of<float>(M, K, F);
+extern "C" int64_t gated_linear_split_sums(int is_bf16, int M, int K, int F, int dx, int dw) {
+    return is_bf16 ? split_sums<bf16>(M, K, F, dx, dw) : split_sums<float>(M, K, F, dx, dw);
 }
 
 extern "C" int launch_gated_linear_bwd(int is_bf16, const void* x, const void* w,
                                        const void* bias, const void* dy, void* dp, void* dx,
-                                       void* dw, void* db, float* part_db, float* part_dw,
-                                       int M, int K, int F, int splits, hipStream_t st) {
-    return is_bf16 ? bwd<bf16>(x, w, bias, dy, dp, dx, dw, db, part_db, part_dw, M, K, F, splits, st)
-                   : bwd<float>(x, w, bias, dy, dp, dx, dw, db, part_db, part_dw, M, K, F, splits, st);
+                                       void* dw, void* db, float* part_db, float* part,
+                                       int M, int K, int F, hipStream_t st) {
+    return is_bf16 ? bwd<bf16>(x, w, bias, dy, dp, dx, dw, db, part_db, part, M, K, F, st)
+                   : bwd<float>(x, w, bias, dy, dp, dx, dw, db, part_db, part, M, K, F, st);
 }
