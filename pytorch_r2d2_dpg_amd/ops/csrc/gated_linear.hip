@@ -443,11 +443,16 @@ join_splits_kernel(const float* __restrict__ part, E* __restrict__ out, int64_t 
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     const int have = n - i < 4 ? (int)(n - i) : 4;
-    float s[4] = {}, v[4];
-    for (int z = 0; z < splits; ++z) {
-        load_run<float, 4>(part + z * n + i, have, v);
+    float s[4] = {}, v[8][4];
+    for (int z0 = 0; z0 < splits; z0 += 8) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s[q] += v[q];
+        for (int z = 0; z < 8; ++z)
+            if (z0 + z < splits) load_run<float, 4>(part + (z0 + z) * n + i, have, v[z]);
+#pragma unroll
+        for (int z = 0; z < 8; ++z)
+            if (z0 + z < splits)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) s[q] += v[z][q];
     }
     E o[4];
 #pragma unroll
@@ -457,20 +462,26 @@ join_splits_kernel(const float* __restrict__ part, E* __restrict__ out, int64_t 
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// The tiles that a product may be cut into, and what a CU reaches with each in
-// a long product (TFLOP/s), measured.
+// The tiles that a product may be cut into: how many blocks of one share a CU,
+// what the CU reaches with them in a long product (TFLOP/s), and the time that
+// one block alone takes for a step of DEPTH, which it spends waiting (us); all
+// measured.
+struct Rate {
+    int blocks;
+    double tflops, alone;
+};
 template <typename E, typename F>
 void each_tile(F&& f) {
     if constexpr (sizeof(E) == 2) {
-        f(Tile<256, 256, 2, 4>(), 4.9);
-        f(Tile<192, 256, 2, 4>(), 4.7);
-        f(Tile<160, 256, 2, 4>(), 4.5);
-        f(Tile<128, 256, 2, 4>(), 4.3);
-        f(Tile<128, 128, 2, 2>(), 3.4);
-        f(Tile<64, 64, 2, 2>(), 1.8);
+        f(Tile<256, 256, 2, 4>(), Rate{1, 4.9, 0});
+        f(Tile<192, 256, 2, 4>(), Rate{1, 4.7, 0});
+        f(Tile<160, 256, 2, 4>(), Rate{1, 4.5, 0});
+        f(Tile<128, 256, 2, 4>(), Rate{1, 4.3, 0});
+        f(Tile<128, 128, 2, 2>(), Rate{2, 3.5, 0.8});
+        f(Tile<64, 64, 2, 2>(), Rate{4, 2.0, 0.5});
     } else {
-        f(Tile<128, 128, 2, 2>(), 0.5);
-        f(Tile<64, 64, 2, 2>(), 0.4);
+        f(Tile<128, 128, 2, 2>(), Rate{2, 0.5, 2.2});
+        f(Tile<64, 64, 2, 2>(), Rate{4, 0.47, 0.75});
     }
 }
 
@@ -480,24 +491,29 @@ struct Cut {
     int bm, bn, splits;
 };
 
-// The cut with the least estimated time: rounds of one tile a CU, each as long
-// as its k takes plus a tile's start and end, plus the splits' way through
-// memory. `wide` is N, or 2F where gate and value columns share a tile.
+// The cut with the least estimated time: what the fullest CU does, plus the
+// splits' way through memory. `wide` is N, or 2F where gate and value columns
+// share a tile.
 template <typename E>
 Cut cut_of(int64_t m, int64_t wide, int64_t k, bool may_split) {
     constexpr int64_t CUS = 256;
     Cut best{0, 0, 1};
     double least = 0;
-    each_tile<E>([&](auto tile, double rate) {
+    if (m < 1) m = 1;  // sums over no rows, for one
+    if (wide < 1) wide = 1;
+    each_tile<E>([&](auto tile, Rate rate) {
         using T = decltype(tile);
         const int64_t tiles = (int64_t)ceil_div(m, T::BM) * ceil_div(wide, T::BN);
         const int64_t steps = ceil_div(k, DEPTH<E>);
         for (int64_t splits = 1; splits <= 64; splits *= 2) {
             if (splits > 1 && (!may_split || steps < 2 * splits)) break;
-            const int64_t rounds = (tiles * splits + CUS - 1) / CUS;
-            const double step = 2.0 * T::BM * T::BN * DEPTH<E> / rate * 1e-6;  // us
+            const int64_t mine = (tiles * splits + CUS - 1) / CUS;  // a CU's blocks
+            const int64_t together = mine < rate.blocks ? mine : rate.blocks;
+            const double shared = together * 2.0 * T::BM * T::BN * DEPTH<E> / rate.tflops * 1e-6;
+            const double step = shared > rate.alone ? shared : rate.alone;
+            const int64_t rounds = (mine + together - 1) / together;
             double us = rounds * (ceil_div(steps, splits) * step + 1.5 + T::BM * T::BN / 32768.0);
-            if (splits > 1) us += 3.0 + splits * m * wide * 8 / 4e6;
+            if (splits > 1) us += 3.0 + splits * m * wide * 8 / 6e6;
             if (best.bm == 0 || us < least) {
                 least = us;
                 best = {T::BM, T::BN, (int)splits};
@@ -528,7 +544,7 @@ int launch(Args<E> p, int splits, hipStream_t st) {
 template <typename E, Lie LA, Lie LB, End END>
 int product(const Args<E>& p, Cut cut, hipStream_t st) {
     int rc = -1;
-    each_tile<E>([&](auto tile, double) {
+    each_tile<E>([&](auto tile, Rate) {
         using T = decltype(tile);
         if (T::BM == cut.bm && T::BN == cut.bn) rc = launch<E, T, LA, LB, END>(p, cut.splits, st);
     });

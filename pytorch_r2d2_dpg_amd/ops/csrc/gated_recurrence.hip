@@ -423,10 +423,10 @@ struct Plan {
 constexpr int WAVES = 4096;
 
 Plan plan_of(int T, int B, int H) {
-    if (T == 0) return {1, 1, 0};  // the state alone
-    const int chunks = (T + CHUNK - 1) / CHUNK;
     const int64_t tiles = ((int64_t)B * ((H + 1) / 2) + 63) / 64;
-    const int64_t most = tiles > 0 ? WAVES / tiles : MAX_WAVES;
+    if (T == 0 || tiles == 0) return {1, 1, 0};  // the state alone, or nothing
+    const int chunks = (T + CHUNK - 1) / CHUNK;
+    const int64_t most = WAVES / tiles;
     int waves = most < 4 ? 4 : most < MAX_WAVES ? (int)most : MAX_WAVES;
     int passes = (chunks + waves - 1) / waves;
     if (tiles * waves * 2 > WAVES || passes < 3) return {(chunks + passes - 1) / passes, 1, passes};

@@ -138,7 +138,7 @@ def gated_recurrence_ref(gates, h0=None, lengths=None):
     y = 0. Returns (y [T,B,H], hT [B,H] in 32 bits at least). Differentiable."""
     wide = torch.promote_types(gates.dtype, torch.float32)
     T, B, H3 = gates.shape
-    f, v, o = gates.to(wide).split(H3 // 3, dim=-1)
+    f, v, o = gates.to(wide).unflatten(-1, (3, H3 // 3)).unbind(2)
     h = gates.new_zeros(B, H3 // 3, dtype=wide) if h0 is None else h0.to(wide)
     ys = []
     for t in range(T):

@@ -88,7 +88,7 @@ def recurrence_oracle(gates, h0, lengths, dy, dhT):
     h = half(dt)
     T, B, H3 = gates.shape
     H = H3 // 3
-    f, v, o = gates.detach().double().cpu().split(H, dim=-1)
+    f, v, o = gates.detach().double().cpu().unflatten(-1, (3, H)).unbind(2)
     state = torch.zeros(B, H).double() if h0 is None else h0.detach().double().cpu()
     dy = torch.zeros(T, B, H).double() if dy is None else dy.double().cpu()
     R = torch.zeros(B, H).double() if dhT is None else dhT.double().cpu()
@@ -137,9 +137,9 @@ def linear_oracle(x, w, b, dy):
     h = half(dt)
     K, F = x.shape[-1], w.shape[0] // 2
     shape = x.shape
-    x, w = x.detach().double().cpu().reshape(-1, K), w.detach().double().cpu()
-    dy = dy.double().cpu().reshape(-1, F)
-    M = x.shape[0]
+    M = shape[:-1].numel()
+    x, w = x.detach().double().cpu().reshape(M, K), w.detach().double().cpu()
+    dy = dy.double().cpu().reshape(M, F)
     p, ep = x @ w.t(), (K + 4) * U * (x.abs() @ w.abs().t())
     if b is not None:
         bias = b.detach().double().cpu()

@@ -141,6 +141,12 @@ def test_recurrence_channels(B, H, dtype):
     run_recurrence(37, B, H, dtype, state=H != 64, seed=B + H)
 
 
+@pytest.mark.parametrize("B, H", [(0, 8), (3, 0), (0, 0)])
+def test_recurrence_without_channels(B, H):
+    for T in (0, 1, 3000):
+        run_recurrence(T, B, H, FP32)
+
+
 @pytest.mark.parametrize("T, B, H", [(3000, 1, 64), (2049, 2, 65), (5000, 3, 8)])
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_recurrence_long(T, B, H, dtype):
@@ -252,6 +258,12 @@ def run_linear(M, K, F, dtype, bias=True, seed=0, shape=None):
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_linear_rows(M, dtype):
     run_linear(M, 72, 80, dtype, seed=M)
+
+
+@pytest.mark.parametrize("M, K, F", [(0, 8, 8), (5, 0, 8), (5, 8, 0), (0, 0, 0)])
+def test_linear_empty(M, K, F):
+    run_linear(M, K, F, BF16)
+    run_linear(M, K, F, FP32, bias=False)
 
 
 @pytest.mark.parametrize("K", [1, 7, 8, 31, 64, 203, 520])
