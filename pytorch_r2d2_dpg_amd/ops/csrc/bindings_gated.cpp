@@ -2,11 +2,15 @@
 // (K9-K11): checks, outputs and workspaces; the kernels sit behind extern "C"
 // launchers as in bindings.cpp.
 //
-// Every entry runs on its first argument's device and that device's current
+// Each operator is one call: checks, the autograd node (in C++: a Python one
+// costs a training step of a small batch several times its kernels) and the
+// launches. It runs on its first argument's device and that device's current
 // stream. Workspaces are allocated per call on that stream, so calls on several
 // streams and captured graphs share none.
 
 #include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -42,41 +46,81 @@ namespace {
 
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 constexpr int64_t MOST = std::numeric_limits<int>::max() / 2;
 
 hipStream_t stream() { return at::hip::getCurrentHIPStream().stream(); }
 
-// On the first argument's device, contiguous, of its type.
 void check_first(const Tensor& t, const char* name) {
     TORCH_CHECK(t.is_cuda(), name, " must be on GPU");
-    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
-    TORCH_CHECK(t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat32, name,
-                " must be bf16 or fp32 (got ", t.scalar_type(), ")");
+    TORCH_CHECK_TYPE(t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat32,
+                     name, " must be bf16 or fp32 (got ", t.scalar_type(), ")");
 }
 
+// An argument after the first one, on whose device it has to be.
 void check(const Tensor& t, const char* name, const Tensor& first, torch::ScalarType dt,
            at::IntArrayRef shape) {
+    TORCH_CHECK_VALUE(t.sizes() == shape, name, " must be ", shape, ", got ", t.sizes());
+    TORCH_CHECK_TYPE(t.scalar_type() == dt, name, " must be ", dt, ", got ", t.scalar_type());
     TORCH_CHECK(t.device() == first.device(), name, " must be on ", first.device());
-    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
-    TORCH_CHECK(t.scalar_type() == dt, name, " must be ", dt, " (got ", t.scalar_type(), ")");
-    TORCH_CHECK(t.sizes() == shape, name, " must have shape ", shape, " (got ", t.sizes(), ")");
+}
+
+OptTensor contiguous(const OptTensor& t) {
+    return t ? OptTensor(t->contiguous()) : t;
+}
+
+// A leaf whose gradient accumulator was made by a graph that still lives keeps
+// that graph's stream. Where that is not the stream being captured, a captured
+// backward pass would wait on a stream outside of the capture, which ends the
+// process. Refused here, while the forward pass is being captured.
+void check_capture(std::initializer_list<OptTensor> inputs) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    (void)hipStreamIsCapturing(stream(), &status);
+    if (status == hipStreamCaptureStatusNone) return;
+    for (const auto& t : inputs) {
+        if (!t || !t->is_leaf() || !t->requires_grad()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node) continue;
+        const auto made_on = node->stream();
+        TORCH_CHECK(!made_on || made_on->id() == at::hip::getCurrentHIPStream().id(),
+                    "an eager graph of a leaf that this capture differentiates is alive: delete "
+                    "its outputs (or detach them) before the capture");
+    }
+}
+
+// Whether a gradient may be asked for: then the leaves are looked at too.
+template <typename... T>
+bool tracked(const T&... t) {
+    if (!torch::GradMode::is_enabled()) return false;
+    const std::initializer_list<OptTensor> all{t...};
+    bool any = false;
+    for (const auto& v : all) any = any || (v && v->requires_grad());
+    if (any) check_capture(all);
+    return any;
+}
+
+// The kernels' gradients are not differentiable themselves: asked for with
+// create_graph, they raise when someone differentiates them, and are no constants.
+variable_list once(variable_list grads, const char* name) {
+    if (!torch::GradMode::is_enabled()) return grads;
+    for (auto& g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true);
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string(name) + " is differentiable once", (int)grads.size());
+    return (*error)(std::move(grads));
 }
 
 const void* ptr(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 int is_bf16(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 ? 1 : 0; }
 
 // ---- K9: layer norm --------------------------------------------------------
-std::tuple<Tensor, Tensor> layer_norm_fwd(Tensor x, Tensor weight, OptTensor bias,
-                                          OptTensor residual, double eps) {
-    check_first(x, "x");
-    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have a last axis to normalise");
+std::tuple<Tensor, Tensor> layer_norm_fwd(const Tensor& x, const Tensor& weight,
+                                          const OptTensor& bias, const OptTensor& residual,
+                                          double eps) {
     const c10::DeviceGuard guard(x.device());
     const int64_t dim = x.size(-1), rows = x.numel() / dim;
-    TORCH_CHECK(dim <= MOST && rows <= MOST, "x is too large");
-    check(weight, "weight", x, x.scalar_type(), {dim});
-    if (bias) check(*bias, "bias", x, x.scalar_type(), {dim});
-    if (residual) check(*residual, "residual", x, x.scalar_type(), x.sizes());
     auto y = torch::empty_like(x);
     Tensor s;
     if (residual) s = torch::empty_like(x);
@@ -87,172 +131,238 @@ std::tuple<Tensor, Tensor> layer_norm_fwd(Tensor x, Tensor weight, OptTensor bia
     return {y, s};
 }
 
-std::tuple<Tensor, Tensor> layer_norm_bwd(Tensor x, OptTensor residual, Tensor weight, Tensor dy,
-                                          OptTensor ds, double eps) {
-    check_first(x, "x");
-    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have a last axis to normalise");
+std::tuple<Tensor, Tensor> layer_norm_bwd(const Tensor& x, const OptTensor& residual,
+                                          const Tensor& weight, const Tensor& dy,
+                                          const OptTensor& ds, double eps) {
     const c10::DeviceGuard guard(x.device());
     const int64_t dim = x.size(-1), rows = x.numel() / dim;
-    TORCH_CHECK(dim <= MOST && rows <= MOST, "x is too large");
-    check(weight, "weight", x, x.scalar_type(), {dim});
-    check(dy, "dy", x, x.scalar_type(), x.sizes());
-    if (residual) check(*residual, "residual", x, x.scalar_type(), x.sizes());
-    if (ds) check(*ds, "ds", x, x.scalar_type(), x.sizes());
     const int parts = norm_bwd_parts(is_bf16(x), rows, (int)dim);
-    const auto f32 = x.options().dtype(torch::kFloat32);
+    const int64_t stats = norm_bwd_stats(is_bf16(x), rows, (int)dim);
     auto dx = torch::empty_like(x);
     auto dwb = torch::empty({2, dim}, x.options());
-    auto part = torch::empty({parts, 2 * dim}, f32);
-    auto stats = torch::empty({norm_bwd_stats(is_bf16(x), rows, (int)dim)}, f32);
+    auto part = torch::empty({parts * 2 * dim + stats}, x.options().dtype(torch::kFloat32));
+    float* sums = part.data_ptr<float>();
     const int rc = launch_norm_bwd(is_bf16(x), x.data_ptr(), ptr(residual), weight.data_ptr(),
-                                   dy.data_ptr(), ptr(ds), dx.data_ptr(), part.data_ptr<float>(),
-                                   stats.data_ptr<float>(), dwb.data_ptr(), rows, (int)dim, parts,
+                                   dy.data_ptr(), ptr(ds), dx.data_ptr(), sums,
+                                   sums + parts * 2 * dim, dwb.data_ptr(), rows, (int)dim, parts,
                                    (float)eps, stream());
     TORCH_CHECK(rc == 0, "layer norm backward launch failed");
     return {dx, dwb};
 }
 
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                                 const OptTensor& bias, const OptTensor& residual, double eps) {
+        auto [y, s] = layer_norm_fwd(x, weight, bias, residual, eps);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->save_for_backward({x, weight, residual ? *residual : Tensor()});
+        return residual ? variable_list{y, s} : variable_list{y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &residual = saved[2];
+        const bool fused = residual.defined();
+        const Tensor dy = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(x);
+        OptTensor ds;
+        if (fused && grads[1].defined()) ds = grads[1].contiguous();
+        auto [dx, dwb] = layer_norm_bwd(x, fused ? OptTensor(residual) : OptTensor(), saved[1], dy,
+                                        ds, ctx->saved_data["eps"].toDouble());
+        return once({dx, dwb[0], ctx->saved_data["bias"].toBool() ? dwb[1] : Tensor(),
+                     fused ? dx : Tensor(), Tensor()}, "layer_norm");
+    }
+};
+
+variable_list layer_norm(const Tensor& x, const Tensor& weight, const OptTensor& bias, double eps,
+                         const OptTensor& residual) {
+    check_first(x, "x");
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x must have a last axis to normalise, got ",
+                      x.sizes());
+    const int64_t dim = x.size(-1);
+    TORCH_CHECK(dim <= MOST && x.numel() / dim <= MOST, "x is too large");
+    check(weight, "weight", x, x.scalar_type(), {dim});
+    if (bias) check(*bias, "bias", x, x.scalar_type(), {dim});
+    if (residual) check(*residual, "residual", x, x.scalar_type(), x.sizes());
+    if (tracked(x, weight, bias, residual))
+        return LayerNorm::apply(x.contiguous(), weight.contiguous(), contiguous(bias),
+                                contiguous(residual), eps);
+    auto [y, s] = layer_norm_fwd(x.contiguous(), weight.contiguous(), contiguous(bias),
+                                 contiguous(residual), eps);
+    return residual ? variable_list{y, s} : variable_list{y};
+}
+
 // ---- K10: gated linear recurrence ------------------------------------------
-std::tuple<Tensor, Tensor, Tensor> gated_recurrence_fwd(Tensor gates, OptTensor h0,
-                                                        OptTensor lengths, bool keep) {
-    check_first(gates, "gates");
-    TORCH_CHECK(gates.dim() == 3 && gates.size(2) % 3 == 0, "gates must be [T, B, 3H]");
+std::tuple<Tensor, Tensor, Tensor> gated_recurrence_fwd(const Tensor& gates, const OptTensor& h0,
+                                                        const OptTensor& lengths, bool keep) {
     const c10::DeviceGuard guard(gates.device());
     const int64_t T = gates.size(0), B = gates.size(1), H = gates.size(2) / 3;
-    // places in a step are counted in 32 bits, of the whole in 64
-    TORCH_CHECK(T <= MOST && B <= MOST && H <= MOST && 3 * B * (H + 1) <= MOST,
-                "gates is too large");
-    if (h0) check(*h0, "h0", gates, torch::kFloat32, {B, H});
-    if (lengths) check(*lengths, "lengths", gates, torch::kInt32, {B});
     const auto f32 = gates.options().dtype(torch::kFloat32);
     auto y = torch::empty({T, B, H}, gates.options());
     auto hT = torch::empty({B, H}, f32);
-    const int64_t chunk = recurrence_chunk();
-    Tensor kept;
+    const int64_t chunk = recurrence_chunk(), maps = recurrence_maps((int)T, (int)B, (int)H);
+    Tensor kept, work;
     if (keep) kept = torch::empty({(T + chunk - 1) / chunk, B, H}, f32);
-    auto maps = torch::empty({recurrence_maps((int)T, (int)B, (int)H)}, f32);
+    if (maps) work = torch::empty({maps}, f32);
     const int rc = launch_recurrence_fwd(
         is_bf16(gates), gates.data_ptr(), (const float*)ptr(h0), (const int*)ptr(lengths),
         y.data_ptr(), hT.data_ptr<float>(), keep ? kept.data_ptr<float>() : nullptr,
-        maps.data_ptr<float>(), (int)T, (int)B, (int)H, stream());
+        maps ? work.data_ptr<float>() : nullptr, (int)T, (int)B, (int)H, stream());
     TORCH_CHECK(rc == 0, "gated recurrence launch failed");
     return {y, hT, kept};
 }
 
-std::tuple<Tensor, Tensor> gated_recurrence_bwd(Tensor gates, Tensor kept, OptTensor lengths,
-                                                Tensor dy, OptTensor dhT) {
-    check_first(gates, "gates");
-    TORCH_CHECK(gates.dim() == 3 && gates.size(2) % 3 == 0, "gates must be [T, B, 3H]");
+std::tuple<Tensor, Tensor> gated_recurrence_bwd(const Tensor& gates, const Tensor& kept,
+                                                const OptTensor& lengths, const Tensor& dy,
+                                                const OptTensor& dhT) {
     const c10::DeviceGuard guard(gates.device());
     const int64_t T = gates.size(0), B = gates.size(1), H = gates.size(2) / 3;
-    const int64_t chunk = recurrence_chunk();
-    check(kept, "kept", gates, torch::kFloat32, {(T + chunk - 1) / chunk, B, H});
-    check(dy, "dy", gates, gates.scalar_type(), {T, B, H});
-    if (dhT) check(*dhT, "dhT", gates, torch::kFloat32, {B, H});
-    if (lengths) check(*lengths, "lengths", gates, torch::kInt32, {B});
+    const int64_t maps = recurrence_maps((int)T, (int)B, (int)H);
     auto dgates = torch::empty_like(gates);
     auto dh0 = torch::empty({B, H}, kept.options());
-    auto maps = torch::empty({recurrence_maps((int)T, (int)B, (int)H)}, kept.options());
+    Tensor work;
+    if (maps) work = torch::empty({maps}, kept.options());
     const int rc = launch_recurrence_bwd(
         is_bf16(gates), gates.data_ptr(), kept.data_ptr<float>(), (const int*)ptr(lengths),
         dy.data_ptr(), (const float*)ptr(dhT), dgates.data_ptr(), dh0.data_ptr<float>(),
-        maps.data_ptr<float>(), (int)T, (int)B, (int)H, stream());
+        maps ? work.data_ptr<float>() : nullptr, (int)T, (int)B, (int)H, stream());
     TORCH_CHECK(rc == 0, "gated recurrence backward launch failed");
     return {dgates, dh0};
 }
 
-// ---- K11: gated linear unit ------------------------------------------------
-struct LinearSizes {
-    int64_t M, K, F;
+struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& gates, const OptTensor& h0,
+                                 const OptTensor& lengths) {
+        auto [y, hT, kept] = gated_recurrence_fwd(gates, h0, lengths, true);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["h0"] = h0.has_value();
+        ctx->save_for_backward({gates, kept, lengths ? *lengths : Tensor()});
+        return {y, hT};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor& gates = saved[0];
+        const Tensor dy = grads[0].defined()
+            ? grads[0].contiguous()
+            : torch::zeros({gates.size(0), gates.size(1), gates.size(2) / 3}, gates.options());
+        OptTensor dhT, lengths;
+        if (grads[1].defined()) dhT = grads[1].contiguous();
+        if (saved[2].defined()) lengths = saved[2];
+        auto [dgates, dh0] = gated_recurrence_bwd(gates, saved[1], lengths, dy, dhT);
+        return once({dgates, ctx->saved_data["h0"].toBool() ? dh0 : Tensor(), Tensor()},
+                    "gated_recurrence");
+    }
 };
 
-LinearSizes check_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const OptTensor& h0,
+                                            const OptTensor& lengths) {
+    check_first(gates, "gates");
+    TORCH_CHECK_VALUE(gates.dim() == 3 && gates.size(2) % 3 == 0,
+                      "gates must be [T, B, 3H], got ", gates.sizes());
+    const int64_t T = gates.size(0), B = gates.size(1), H = gates.size(2) / 3;
+    // places in a step are counted in 32 bits, of the whole in 64
+    TORCH_CHECK(T <= MOST && B <= MOST && H <= MOST && 3 * B * (H + 1) <= MOST,
+                "gates is too large");
+    if (h0) check(*h0, "h0 (the state is not rounded)", gates, torch::kFloat32, {B, H});
+    if (lengths) check(*lengths, "lengths", gates, torch::kInt32, {B});
+    if (tracked(gates, h0)) {
+        auto out = GatedRecurrence::apply(gates.contiguous(), contiguous(h0), contiguous(lengths));
+        return {out[0], out[1]};
+    }
+    auto [y, hT, kept] =
+        gated_recurrence_fwd(gates.contiguous(), contiguous(h0), contiguous(lengths), false);
+    return {y, hT};
+}
+
+// ---- K11: gated linear unit ------------------------------------------------
+struct LinearSizes {
+    int M, K, F;
+    std::vector<int64_t> out;
+};
+
+LinearSizes sizes_of(const Tensor& x, const Tensor& weight) {
+    auto out = x.sizes().vec();
+    int64_t M = 1;
+    for (size_t i = 0; i + 1 < out.size(); ++i) M *= out[i];
+    const int64_t K = out.back(), F = weight.size(0) / 2;
+    out.back() = F;
+    return {(int)M, (int)K, (int)F, out};
+}
+
+Tensor gated_linear_fwd(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+    const c10::DeviceGuard guard(x.device());
+    const auto n = sizes_of(x, weight);
+    auto y = torch::empty(n.out, x.options());
+    const int rc = launch_gated_linear_fwd(is_bf16(x), x.data_ptr(), weight.data_ptr(), ptr(bias),
+                                           y.data_ptr(), n.M, n.K, n.F, stream());
+    TORCH_CHECK(rc == 0, "gated linear launch failed");
+    return y;
+}
+
+variable_list gated_linear_bwd(const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                               const Tensor& dy, bool need_x, bool need_w, bool need_b) {
+    const c10::DeviceGuard guard(x.device());
+    const auto n = sizes_of(x, weight);
+    const int half = is_bf16(x);
+    const int64_t rows = need_b ? gated_linear_bias_parts(half, n.M, n.K, n.F) : 0;
+    const int64_t splits = gated_linear_split_sums(half, n.M, n.K, n.F, need_x, need_w);
+    auto dp = torch::empty({n.M, 2 * (int64_t)n.F}, x.options());
+    auto part = torch::empty({splits + rows * 2 * n.F}, x.options().dtype(torch::kFloat32));
+    Tensor dx, dw, db;
+    if (need_x) dx = torch::empty_like(x);
+    if (need_w) dw = torch::empty_like(weight);
+    if (need_b) db = torch::empty({2 * (int64_t)n.F}, x.options());
+    float* sums = part.data_ptr<float>();  // the splits', 16-byte pieces of them, first
+    const int rc = launch_gated_linear_bwd(
+        half, x.data_ptr(), weight.data_ptr(), ptr(bias), dy.data_ptr(), dp.data_ptr(),
+        need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
+        need_b ? db.data_ptr() : nullptr, sums + splits, sums, n.M, n.K, n.F, stream());
+    TORCH_CHECK(rc == 0, "gated linear backward launch failed");
+    return {dx, dw, db};
+}
+
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                                 const OptTensor& bias) {
+        ctx->save_for_backward({x, weight, bias ? *bias : Tensor()});
+        return {gated_linear_fwd(x, weight, bias)};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        OptTensor bias;
+        if (saved[2].defined()) bias = saved[2];
+        return once(gated_linear_bwd(saved[0], saved[1], bias, grads[0].contiguous(),
+                                     ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                     bias && ctx->needs_input_grad(2)), "gated_linear");
+    }
+};
+
+Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
     check_first(x, "x");
-    TORCH_CHECK(x.dim() >= 1, "x must have a last axis");
-    TORCH_CHECK(weight.dim() == 2 && weight.size(0) % 2 == 0, "weight must be [2F, K]");
+    TORCH_CHECK_VALUE(x.dim() >= 1, "x must have a last axis");
+    TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) % 2 == 0,
+                      "weight must be [2F, K], got ", weight.sizes());
     const int64_t K = x.size(-1), F = weight.size(0) / 2;
     check(weight, "weight", x, x.scalar_type(), {2 * F, K});
     if (bias) check(*bias, "bias", x, x.scalar_type(), {2 * F});
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
     // tiles of 64 by 64 at the least lie on one grid axis
+    TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST / 2, "x or weight is too large");
     const int64_t m = M / 64 + 1, k = K / 64 + 1, f = 2 * F / 64 + 1;
-    TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST / 2 && m * f <= MOST && m * k <= MOST &&
-                    k * f <= MOST, "x or weight is too large");
-    return {M, K, F};
-}
-
-Tensor gated_linear_fwd(Tensor x, Tensor weight, OptTensor bias) {
-    const auto n = check_linear(x, weight, bias);
-    const c10::DeviceGuard guard(x.device());
-    auto shape = x.sizes().vec();
-    shape.back() = n.F;
-    auto y = torch::empty(shape, x.options());
-    const int rc = launch_gated_linear_fwd(is_bf16(x), x.data_ptr(), weight.data_ptr(), ptr(bias),
-                                           y.data_ptr(), (int)n.M, (int)n.K, (int)n.F, stream());
-    TORCH_CHECK(rc == 0, "gated linear launch failed");
-    return y;
-}
-
-std::tuple<Tensor, Tensor, Tensor> gated_linear_bwd(Tensor x, Tensor weight, OptTensor bias,
-                                                    Tensor dy, bool need_x, bool need_w,
-                                                    bool need_b) {
-    const auto n = check_linear(x, weight, bias);
-    const c10::DeviceGuard guard(x.device());
-    auto shape = x.sizes().vec();
-    shape.back() = n.F;
-    check(dy, "dy", x, x.scalar_type(), shape);
-    const auto f32 = x.options().dtype(torch::kFloat32);
-    auto dp = torch::empty({n.M, 2 * n.F}, x.options());
-    Tensor dx, dw, db, part_db;
-    const int M = (int)n.M, K = (int)n.K, F = (int)n.F, half = is_bf16(x);
-    if (need_x) dx = torch::empty_like(x);
-    if (need_w) dw = torch::empty_like(weight);
-    if (need_b) {
-        db = torch::empty({2 * n.F}, x.options());
-        part_db = torch::empty({gated_linear_bias_parts(half, M, K, F), 2 * n.F}, f32);
-    }
-    auto part = torch::empty({gated_linear_split_sums(half, M, K, F, need_x, need_w)}, f32);
-    const int rc = launch_gated_linear_bwd(
-        half, x.data_ptr(), weight.data_ptr(), ptr(bias), dy.data_ptr(), dp.data_ptr(),
-        need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
-        need_b ? db.data_ptr() : nullptr, need_b ? part_db.data_ptr<float>() : nullptr,
-        part.data_ptr<float>(), M, K, F, stream());
-    TORCH_CHECK(rc == 0, "gated linear backward launch failed");
-    return {dx, dw, db};
-}
-
-// A leaf whose gradient accumulator was made by a graph that still lives keeps
-// that graph's stream. Where that is not the stream being captured, a captured
-// backward pass would wait on a stream outside of the capture, which ends the
-// process. Refused here, while the forward pass is being captured.
-void check_capture(const std::vector<OptTensor>& inputs) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    (void)hipStreamIsCapturing(stream(), &status);
-    if (status == hipStreamCaptureStatusNone) return;
-    for (const auto& t : inputs) {
-        if (!t.has_value() || !t->defined() || !t->is_leaf() || !t->requires_grad()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (!node) continue;
-        const auto made_on = node->stream();
-        TORCH_CHECK(!made_on || made_on->id() == at::hip::getCurrentHIPStream().id(),
-                    "an eager graph of a leaf that this capture differentiates is alive: delete "
-                    "its outputs (or detach them) before the capture");
-    }
+    TORCH_CHECK(m * f <= MOST && m * k <= MOST && k * f <= MOST, "x or weight is too large");
+    if (tracked(x, weight, bias))
+        return GatedLinear::apply(x.contiguous(), weight.contiguous(), contiguous(bias))[0];
+    return gated_linear_fwd(x.contiguous(), weight.contiguous(), contiguous(bias));
 }
 
 }  // namespace
 
 void bind_gated(py::module_& m) {
-    m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm forward (K9)", py::arg("x"),
-          py::arg("weight"), py::arg("bias"), py::arg("residual"), py::arg("eps"));
-    m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward (K9)");
-    m.def("gated_recurrence_fwd", &gated_recurrence_fwd, "gated linear recurrence forward (K10)",
-          py::arg("gates"), py::arg("h0"), py::arg("lengths"), py::arg("keep"));
-    m.def("gated_recurrence_bwd", &gated_recurrence_bwd,
-          "gated linear recurrence backward (K10)");
-    m.def("gated_linear_fwd", &gated_linear_fwd, "gated linear unit forward (K11)");
-    m.def("gated_linear_bwd", &gated_linear_bwd, "gated linear unit backward (K11)");
-    m.def("check_capture", &check_capture,
-          "refuse to capture a graph over leaves of a live eager graph");
+    m.def("layer_norm", &layer_norm, "layer norm, [y] or [y, x + residual] (K9)", py::arg("x"),
+          py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("residual"));
+    m.def("gated_recurrence", &gated_recurrence, "gated linear recurrence, (y, hT) (K10)",
+          py::arg("gates"), py::arg("h0"), py::arg("lengths"));
+    m.def("gated_linear", &gated_linear, "gated linear unit (K11)", py::arg("x"),
+          py::arg("weight"), py::arg("bias"));
 }

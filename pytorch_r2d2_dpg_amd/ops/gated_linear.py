@@ -13,25 +13,9 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip_ext
 from .reference import gated_linear_ref
-
-
-class _GatedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        ctx.save_for_backward(x, weight, bias)
-        return hip_ext().gated_linear_fwd(x, weight, bias)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad
-        return hip_ext().gated_linear_bwd(x, weight, bias, dy.contiguous(),
-                                          need_x, need_w, need_b)
 
 
 def gated_linear(
@@ -43,6 +27,8 @@ def gated_linear(
 
     weight and bias share x's type. Differentiable once in every tensor.
     """
+    if x.is_cuda:
+        return hip_ext().gated_linear(x, weight, bias)
     if x.dim() == 0:
         raise ValueError("x must have a last axis")
     if weight.dim() != 2 or weight.shape[0] % 2 or weight.shape[1] != x.shape[-1]:
@@ -52,11 +38,4 @@ def gated_linear(
     given = [t for t in (x, weight, bias) if t is not None]
     if any(t.dtype != x.dtype for t in given):
         raise TypeError(f"dtype mismatch: {[t.dtype for t in given]}")
-    if not x.is_cuda:
-        return gated_linear_ref(x, weight, bias)
-    x, weight = x.contiguous(), weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-        hip_ext().check_capture(given)
-        return _GatedLinear.apply(x, weight, bias)
-    return hip_ext().gated_linear_fwd(x, weight, bias)
+    return gated_linear_ref(x, weight, bias)

@@ -14,30 +14,9 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip_ext
 from .reference import gated_recurrence_ref
-
-
-class _GatedRecurrence(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gates, h0, lengths):
-        y, hT, kept = hip_ext().gated_recurrence_fwd(gates, h0, lengths, True)
-        ctx.set_materialize_grads(False)
-        ctx.has_h0 = h0 is not None
-        ctx.save_for_backward(gates, kept, lengths)
-        return y, hT
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dhT):
-        gates, kept, lengths = ctx.saved_tensors
-        if dy is None:
-            dy = gates.new_zeros(gates.shape[0], gates.shape[1], gates.shape[2] // 3)
-        dgates, dh0 = hip_ext().gated_recurrence_bwd(
-            gates, kept, lengths, dy.contiguous(), None if dhT is None else dhT.contiguous())
-        return dgates, dh0 if ctx.has_h0 else None, None
 
 
 def gated_recurrence(
@@ -52,6 +31,8 @@ def gated_recurrence(
     y is 0, their gates have no effect and no gradient. Values outside [0, T]
     count as the nearer end. Differentiable once in gates and h0.
     """
+    if gates.is_cuda:
+        return hip_ext().gated_recurrence(gates, h0, lengths)
     if gates.dim() != 3 or gates.shape[2] % 3:
         raise ValueError(f"gates must be [T, B, 3H], got {tuple(gates.shape)}")
     B, H = gates.shape[1], gates.shape[2] // 3
@@ -66,14 +47,4 @@ def gated_recurrence(
             raise ValueError(f"lengths must be [{B}], got {tuple(lengths.shape)}")
         if lengths.dtype != torch.int32:
             raise TypeError(f"lengths must be int32, got {lengths.dtype}")
-    if not gates.is_cuda:
-        return gated_recurrence_ref(gates, h0, lengths)
-    given = (gates, h0)
-    gates = gates.contiguous()
-    h0 = None if h0 is None else h0.contiguous()
-    lengths = None if lengths is None else lengths.contiguous()
-    if torch.is_grad_enabled() and (gates.requires_grad or (h0 is not None and h0.requires_grad)):
-        hip_ext().check_capture(given)
-        return _GatedRecurrence.apply(gates, h0, lengths)
-    y, hT, _ = hip_ext().gated_recurrence_fwd(gates, h0, lengths, False)
-    return y, hT
+    return gated_recurrence_ref(gates, h0, lengths)

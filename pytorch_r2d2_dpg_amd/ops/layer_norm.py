@@ -4,7 +4,8 @@
 
 over the last axis: one launch forward, two backward (rows, then the fixed-order
 sum of the weight's and bias's gradients). Sums and statistics are in 32 bits.
-On GPU the HIP kernel runs (bf16 or fp32), on CPU the differentiable reference.
+On GPU the HIP kernels run (bf16 or fp32; checks and gradient are the binding's),
+on CPU the differentiable reference.
 """
 
 from __future__ import annotations
@@ -12,29 +13,9 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip_ext
 from .reference import layer_norm_ref
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, eps):
-        y, s = hip_ext().layer_norm_fwd(x, weight, bias, residual, eps)
-        ctx.set_materialize_grads(False)
-        ctx.has_bias, ctx.fused, ctx.eps = bias is not None, residual is not None, eps
-        ctx.save_for_backward(x, weight, residual)
-        return y if residual is None else (y, s)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, ds=None):
-        x, weight, residual = ctx.saved_tensors
-        dy = torch.zeros_like(x) if dy is None else dy.contiguous()
-        ds = None if ds is None else ds.contiguous()
-        dx, dwb = hip_ext().layer_norm_bwd(x, residual, weight, dy, ds, ctx.eps)
-        return dx, dwb[0], dwb[1] if ctx.has_bias else None, dx if ctx.fused else None, None
 
 
 def layer_norm(
@@ -50,6 +31,9 @@ def layer_norm(
     shape and type, which weight, bias and residual share. Differentiable once
     in every tensor.
     """
+    if x.is_cuda:
+        out = hip_ext().layer_norm(x, weight, bias, eps, residual)
+        return out[0] if residual is None else (out[0], out[1])
     D = x.shape[-1] if x.dim() else 0
     if D == 0:
         raise ValueError(f"x must have a last axis to normalise (got {tuple(x.shape)})")
@@ -61,13 +45,4 @@ def layer_norm(
     given = [t for t in (x, weight, bias, residual) if t is not None]
     if any(t.dtype != x.dtype for t in given):
         raise TypeError(f"dtype mismatch: {[t.dtype for t in given]}")
-    if not x.is_cuda:
-        return layer_norm_ref(x, weight, bias, eps, residual)
-    x, weight = x.contiguous(), weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-        hip_ext().check_capture(given)
-        return _LayerNorm.apply(x, weight, bias, residual, float(eps))
-    y, s = hip_ext().layer_norm_fwd(x, weight, bias, residual, float(eps))
-    return y if residual is None else (y, s)
+    return layer_norm_ref(x, weight, bias, eps, residual)

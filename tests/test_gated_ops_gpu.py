@@ -309,22 +309,52 @@ def test_linear_keeps_rows_apart():
 
 
 # ----------------------------------------------------- refusals, streams, graphs
-def test_gpu_refusals():
-    x, w = rand(3, 8), rand(8, seed=1)
-    with pytest.raises(RuntimeError):
-        layer_norm(x.half(), w.half())
-    with pytest.raises(RuntimeError):
-        layer_norm(x, w.cpu())
-    with pytest.raises(RuntimeError):
-        gated_recurrence(rand(2, 3, 6).half())
-    with pytest.raises(RuntimeError):
-        gated_recurrence(rand(2, 3, 6), None, torch.zeros(3, dtype=torch.int32))
-    with pytest.raises(RuntimeError):
-        gated_linear(x, rand(4, 8).cpu())
-    y = layer_norm(x.requires_grad_(True), w)
-    g = torch.autograd.grad(y.sum(), x, create_graph=True)[0]
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(g.sum(), x)
+def i32(*shape, device="cuda"):
+    return torch.zeros(*shape, dtype=torch.int32, device=device)
+
+
+@pytest.mark.parametrize("call, error", [
+    (lambda: layer_norm(rand(3, 8).half(), rand(8).half()), TypeError),
+    (lambda: layer_norm(rand(3, 8), rand(8, dtype=BF16)), TypeError),
+    (lambda: layer_norm(rand(3, 8), rand(8).cpu()), RuntimeError),
+    (lambda: layer_norm(rand(3, 8), rand(8), residual=rand(3, 8).cpu()), RuntimeError),
+    (lambda: layer_norm(rand(3, 8), rand(8), residual=rand(1, 8)), ValueError),
+    (lambda: layer_norm(rand(3, 8), rand(7)), ValueError),
+    (lambda: layer_norm(rand(3, 8), rand(8), rand(7)), ValueError),
+    (lambda: layer_norm(rand(3, 0), rand(0)), ValueError),
+    (lambda: layer_norm(rand(1)[0], rand(1)), ValueError),
+    (lambda: gated_recurrence(rand(2, 3, 6).half()), TypeError),
+    (lambda: gated_recurrence(rand(2, 3, 6).double()), TypeError),
+    (lambda: gated_recurrence(rand(2, 3, 7)), ValueError),
+    (lambda: gated_recurrence(rand(3, 6)), ValueError),
+    (lambda: gated_recurrence(rand(2, 3, 6), rand(3, 3)), ValueError),
+    (lambda: gated_recurrence(rand(2, 3, 6), rand(3, 2, dtype=BF16)), TypeError),
+    (lambda: gated_recurrence(rand(2, 3, 6), rand(3, 2).cpu()), RuntimeError),
+    (lambda: gated_recurrence(rand(2, 3, 6), None, i32(2)), ValueError),
+    (lambda: gated_recurrence(rand(2, 3, 6), None, i32(3).long()), TypeError),
+    (lambda: gated_recurrence(rand(2, 3, 6), None, i32(3, device="cpu")), RuntimeError),
+    (lambda: gated_linear(rand(3, 8), rand(4, 8).cpu()), RuntimeError),
+    (lambda: gated_linear(rand(3, 8).half(), rand(4, 8).half()), TypeError),
+    (lambda: gated_linear(rand(3, 8), rand(4, 8, dtype=BF16)), TypeError),
+    (lambda: gated_linear(rand(3, 8), rand(5, 8)), ValueError),
+    (lambda: gated_linear(rand(3, 8), rand(4, 7)), ValueError),
+    (lambda: gated_linear(rand(3, 8), rand(4, 8), rand(2)), ValueError),
+    (lambda: gated_linear(rand(1)[0], rand(4, 1)), ValueError),
+])
+def test_gpu_refusals(call, error):
+    with pytest.raises(error):
+        call()
+
+
+def test_second_derivatives_are_refused():
+    x, w = rand(3, 8).requires_grad_(True), rand(8, seed=1)
+    for op in (lambda: layer_norm(x, w), lambda: gated_linear(x, rand(6, 8, seed=2)),
+               lambda: gated_recurrence(x.view(1, 1, 24))[0]):
+        g = torch.autograd.grad(op().square().sum(), x, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            g.sum().backward()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
 
 
 def block(p, gates_of):
