@@ -49,6 +49,7 @@ def flagship_config(args) -> Config:
         cfg.model.hidden_size = args.hidden
         cfg.model.trunk_sizes = (args.hidden, args.hidden)
     cfg.model.dtype = args.dtype
+    cfg.model.core = args.core
     cfg.replay.seq_len = args.seq_len
     cfg.replay.burn_in = args.burn_in
     cfg.replay.n_step = 5
@@ -103,6 +104,8 @@ def main() -> int:
     p.add_argument("--hidden", type=int, default=None,
                    help="LSTM hidden (default: 512; pixel: 256)")
     p.add_argument("--dtype", type=str, default="bf16", choices=["bf16", "fp32"])
+    p.add_argument("--core", type=str, default="lstm", choices=["lstm", "gated"],
+                   help="recurrent core of the nets (default: the LSTM)")
     p.add_argument("--replay-capacity", type=int, default=None)
     p.add_argument("--fp8-obs", action="store_true",
                    help="store observations fp8 e4m3 in the replay shard (K7)")
@@ -205,6 +208,8 @@ def main() -> int:
         model_desc = ("R2D2-DPG " + args.env + " (obs "
                       + str(spec.obs_shape[0]) + ", act " + str(spec.action_dim)
                       + "), LSTM H=" + str(args.hidden) + " trunk 2x" + str(args.hidden))
+    if args.core != "lstm":
+        model_desc = model_desc.replace("LSTM", "GatedCore")
     if rank == 0:
         out = {
             "metric": "learner transitions/sec (whole node), " + args.env,

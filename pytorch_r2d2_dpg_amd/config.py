@@ -37,6 +37,7 @@ class ModelConfig:
     trunk_sizes: tuple = (256, 256)  # MLP trunk layer widths (state obs)
     conv_channels: tuple = (32, 64, 64)  # DQN-style conv stack for 84x84 pixels
     dtype: str = "fp32"             # learner compute dtype: fp32 | bf16
+    core: str = "lstm"              # recurrent core: lstm | gated (models/gated.py)
 
 
 @dataclass

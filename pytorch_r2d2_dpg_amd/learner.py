@@ -149,7 +149,8 @@ class Learner:
         # residency instead (+3% measured; parameter-equivalent to the
         # autograd path, test_pair_bwd_step_matches_default).
         _H = cfg.model.hidden_size
-        self._pair_bwd = (overlap_ok and self.dtype == torch.bfloat16
+        self._lstm = cfg.model.core == "lstm"  # the paired launches are the LSTM's
+        self._pair_bwd = (overlap_ok and self._lstm and self.dtype == torch.bfloat16
                           and _H >= 64 and (_H & (_H - 1)) == 0  # px geometry
                           and not os.environ.get("R2D2_NO_PAIR_BWD"))
         if self._pair_bwd:
@@ -197,7 +198,8 @@ class Learner:
         reward = batch["reward"]                                   # [B, L] fp32
         done = batch["done"]                                       # [B, L] fp32
         weight = batch["weight"]                                   # [B] fp32
-        st = batch["state"].to(self.dtype)                         # [B, 4, H]
+        # [B, 4, H]; the gated core's state stays in 32 bits
+        st = batch["state"].to(self.dtype if self._lstm else torch.float32)
         h_a, c_a = st[:, 0].contiguous(), st[:, 1].contiguous()
         h_c, c_c = st[:, 2].contiguous(), st[:, 3].contiguous()
         length = batch.get("length")
@@ -221,6 +223,11 @@ class Learner:
         bi = self.burn_in
         if bi == 0:
             return h_a, c_a, h_c, c_c
+        if not self._lstm:
+            with torch.no_grad():
+                _, st_a = self.actor(obs[:bi], (h_a, c_a))
+                _, st_c = self.critic(obs[:bi], action[:bi], (h_c, c_c))
+            return *st_a, *st_c
         with torch.no_grad():
             feat_a = self.actor.trunk(obs[:bi])
             feat_c = torch.cat([self.critic.trunk(obs[:bi]), action[:bi]], dim=-1)
@@ -384,23 +391,30 @@ class Learner:
         # target-critic unroll which consumes mu_t (main stream; balances
         # the side stream's actor-chain length)
         ta = self.target_actor
+        if self._lstm:
+            with torch.no_grad():
+                feat_ta = ta.trunk(obs[bi:bi + Tn])
+            feat_cf = self.critic.trunk(obs[bi:bi + T])
+            x_cf = torch.cat([feat_cf, action[bi:bi + T]], dim=-1)
+            hs_ta, _, _, hs_cf, _, _ = lstm_seq_pair_halfgrad(
+                feat_ta, h_a2, c_a2,
+                ta.lstm.weight_x, ta.lstm.weight_h, ta.lstm.bias,
+                x_cf, h_c2.detach(), c_c2.detach(),
+                self.critic.lstm.weight_x, self.critic.lstm.weight_h,
+                self.critic.lstm.bias)
+            Hs = ta.hidden_size
+            with torch.no_grad():
+                mu_t = (torch.tanh(ta.head(hs_ta.reshape(-1, Hs)))
+                        .view(Tn, -1, ta.action_dim) * ta.action_scale)
+            q_online = self.critic.head(hs_cf.reshape(-1, Hs)).view(T, -1)
+        else:
+            with torch.no_grad():
+                mu_t, _ = ta(obs[bi:bi + Tn], (h_a2, c_a2))
+            q_online, _ = self.critic(obs[bi:bi + T], action[bi:bi + T],
+                                      (h_c2.detach(), c_c2.detach()))
         with torch.no_grad():
-            feat_ta = ta.trunk(obs[bi:bi + Tn])
-        feat_cf = self.critic.trunk(obs[bi:bi + T])
-        x_cf = torch.cat([feat_cf, action[bi:bi + T]], dim=-1)
-        hs_ta, _, _, hs_cf, _, _ = lstm_seq_pair_halfgrad(
-            feat_ta, h_a2, c_a2,
-            ta.lstm.weight_x, ta.lstm.weight_h, ta.lstm.bias,
-            x_cf, h_c2.detach(), c_c2.detach(),
-            self.critic.lstm.weight_x, self.critic.lstm.weight_h,
-            self.critic.lstm.bias)
-        Hs = ta.hidden_size
-        with torch.no_grad():
-            mu_t = (torch.tanh(ta.head(hs_ta.reshape(-1, Hs)))
-                    .view(Tn, -1, ta.action_dim) * ta.action_scale)
             qt, _ = self.target_critic(obs[bi:bi + Tn], mu_t, (h_c2, c_c2))
             q_boot = qt[self.n_step:self.n_step + T].transpose(0, 1).float()
-        q_online = self.critic.head(hs_cf.reshape(-1, Hs)).view(T, -1)
         q_online_bt = q_online.transpose(0, 1).float()  # [B, T]
         with torch.no_grad():
             y, td_abs, prio = td_targets_and_priorities(

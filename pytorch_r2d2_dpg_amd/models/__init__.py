@@ -1,4 +1,5 @@
 from .lstm import FusedLSTM
+from .gated import GatedCore
 from .actor_critic import ActorNet, CriticNet, make_models
 
-__all__ = ["FusedLSTM", "ActorNet", "CriticNet", "make_models"]
+__all__ = ["FusedLSTM", "GatedCore", "ActorNet", "CriticNet", "make_models"]

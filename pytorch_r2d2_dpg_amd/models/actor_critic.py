@@ -4,6 +4,8 @@ ActorNet : obs -> trunk (MLP, or Conv stack for 84x84 pixels) -> FusedLSTM
            -> Linear -> tanh * action_scale
 CriticNet: concat(obs_features, action) -> FusedLSTM -> Linear -> Q scalar
 
+``core="gated"`` puts the GatedCore (models/gated.py) in the FusedLSTM's place.
+
 Both expose sequence form ``forward(x, state)`` over [T, B, ...] and a
 single-step ``step`` for actor rollouts; recurrent state is (h, c).
 Target copies are deep copies updated by Polyak (ops/polyak.py).
@@ -17,6 +19,7 @@ from typing import Optional
 import torch
 from torch import nn
 
+from .gated import GatedCore
 from .lstm import FusedLSTM, State
 
 
@@ -75,16 +78,36 @@ class _TrunkEncoder(nn.Module):
         return feat.view(T, B, -1)
 
 
-class ActorNet(nn.Module):
+CORES = {"lstm": FusedLSTM, "gated": GatedCore}
+
+
+class _Recurrent(nn.Module):
+    """The recurrent core of a net, by its name: ``lstm`` or ``gated``."""
+
+    def _make_core(self, core: str, input_size: int, hidden_size: int) -> None:
+        if core not in CORES:
+            raise ValueError(f"unknown model.core {core!r}: one of {sorted(CORES)}")
+        self.core_name = core
+        self.add_module(core, CORES[core](input_size, hidden_size))
+
+    @property
+    def core(self):
+        return getattr(self, self.core_name)
+
+    def zero_state(self, batch: int, device=None, dtype=None) -> State:
+        return self.core.zero_state(batch, device, dtype)
+
+
+class ActorNet(_Recurrent):
     def __init__(self, obs_shape, action_dim: int, action_scale: float = 1.0,
                  hidden_size: int = 256, trunk_sizes=(256, 256),
-                 conv_channels=(32, 64, 64), pixel: bool = False):
+                 conv_channels=(32, 64, 64), pixel: bool = False, core: str = "lstm"):
         super().__init__()
         self.action_dim = action_dim
         self.action_scale = action_scale
         self.hidden_size = hidden_size
         self.trunk = _TrunkEncoder(obs_shape, trunk_sizes, conv_channels, pixel)
-        self.lstm = FusedLSTM(self.trunk.out_dim, hidden_size)
+        self._make_core(core, self.trunk.out_dim, hidden_size)
         self.head = nn.Linear(hidden_size, action_dim)
         # DDPG-paper head init (+-3e-3): keeps initial actions near 0 so the
         # tanh does not saturate before the critic is informative (saturated
@@ -93,13 +116,10 @@ class ActorNet(nn.Module):
             self.head.weight.uniform_(-3e-3, 3e-3)
             self.head.bias.zero_()
 
-    def zero_state(self, batch: int, device=None, dtype=None) -> State:
-        return self.lstm.zero_state(batch, device, dtype)
-
     def forward(self, obs: torch.Tensor, state: Optional[State] = None):
         """obs: [T, B, ...] -> (action [T, B, A], (h, c))."""
         feat = self.trunk(obs)
-        h_seq, st = self.lstm(feat, state)
+        h_seq, st = self.core(feat, state)
         a = torch.tanh(self.head(h_seq.reshape(-1, self.hidden_size)))
         return a.view(h_seq.shape[0], h_seq.shape[1], -1) * self.action_scale, st
 
@@ -108,28 +128,25 @@ class ActorNet(nn.Module):
         return a[0], st
 
 
-class CriticNet(nn.Module):
+class CriticNet(_Recurrent):
     def __init__(self, obs_shape, action_dim: int,
                  hidden_size: int = 256, trunk_sizes=(256, 256),
-                 conv_channels=(32, 64, 64), pixel: bool = False):
+                 conv_channels=(32, 64, 64), pixel: bool = False, core: str = "lstm"):
         super().__init__()
         self.hidden_size = hidden_size
         self.trunk = _TrunkEncoder(obs_shape, trunk_sizes, conv_channels, pixel)
-        self.lstm = FusedLSTM(self.trunk.out_dim + action_dim, hidden_size)
+        self._make_core(core, self.trunk.out_dim + action_dim, hidden_size)
         self.head = nn.Linear(hidden_size, 1)
         with torch.no_grad():
             self.head.weight.uniform_(-3e-3, 3e-3)
             self.head.bias.zero_()
-
-    def zero_state(self, batch: int, device=None, dtype=None) -> State:
-        return self.lstm.zero_state(batch, device, dtype)
 
     def forward(self, obs: torch.Tensor, action: torch.Tensor,
                 state: Optional[State] = None):
         """obs [T,B,...], action [T,B,A] -> (q [T,B], (h,c))."""
         feat = self.trunk(obs)
         x = torch.cat([feat, action], dim=-1)
-        h_seq, st = self.lstm(x, state)
+        h_seq, st = self.core(x, state)
         q = self.head(h_seq.reshape(-1, self.hidden_size))
         return q.view(h_seq.shape[0], h_seq.shape[1]), st
 
@@ -142,7 +159,8 @@ class CriticNet(nn.Module):
 def make_models(spec, model_cfg, device="cpu", dtype=torch.float32):
     """Build (actor, critic, target_actor, target_critic) for an EnvSpec."""
     kw = dict(hidden_size=model_cfg.hidden_size, trunk_sizes=tuple(model_cfg.trunk_sizes),
-              conv_channels=tuple(model_cfg.conv_channels), pixel=spec.pixel)
+              conv_channels=tuple(model_cfg.conv_channels), pixel=spec.pixel,
+              core=getattr(model_cfg, "core", "lstm"))
     actor = ActorNet(spec.obs_shape, spec.action_dim, spec.action_scale, **kw)
     critic = CriticNet(spec.obs_shape, spec.action_dim, **kw)
     actor = actor.to(device=device, dtype=dtype)

@@ -72,7 +72,7 @@ OptTensor contiguous(const OptTensor& t) {
 }
 
 // A leaf whose gradient accumulator was made by a graph that still lives keeps
-// that graph's stream. Where that is not the stream being captured, a captured
+// that graph's stream. Where that is not a stream of the capture, a captured
 // backward pass would wait on a stream outside of the capture, which ends the
 // process. Refused here, while the forward pass is being captured.
 void check_capture(std::initializer_list<OptTensor> inputs) {
@@ -84,7 +84,14 @@ void check_capture(std::initializer_list<OptTensor> inputs) {
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         if (!node) continue;
         const auto made_on = node->stream();
-        TORCH_CHECK(!made_on || made_on->id() == at::hip::getCurrentHIPStream().id(),
+        if (!made_on) continue;
+        bool outside = made_on->id() == 0;  // the default stream is never captured
+        if (!outside) {
+            const at::hip::HIPStream made(at::hip::HIPStream::UNCHECKED, *made_on);
+            (void)hipStreamIsCapturing(made.stream(), &status);
+            outside = status == hipStreamCaptureStatusNone;
+        }
+        TORCH_CHECK(!outside,
                     "an eager graph of a leaf that this capture differentiates is alive: delete "
                     "its outputs (or detach them) before the capture");
     }
