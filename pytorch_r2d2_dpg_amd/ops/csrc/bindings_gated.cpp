@@ -358,6 +358,9 @@ Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
     TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST / 2, "x or weight is too large");
     const int64_t m = M / 64 + 1, k = K / 64 + 1, f = 2 * F / 64 + 1;
     TORCH_CHECK(m * f <= MOST && m * k <= MOST && k * f <= MOST, "x or weight is too large");
+    // a tile's places are counted in 32 bits from its first: 256 rows, or a gate's
+    // row and its value's
+    TORCH_CHECK((F + 256) * K <= MOST && 512 * F <= MOST, "weight is too large");
     if (tracked(x, weight, bias))
         return GatedLinear::apply(x.contiguous(), weight.contiguous(), contiguous(bias))[0];
     return gated_linear_fwd(x.contiguous(), weight.contiguous(), contiguous(bias));

@@ -25,8 +25,9 @@ using u4 = __attribute__((ext_vector_type(4))) unsigned int;
 
 // Tiles are handled in pieces of 16 bytes: PIECE elements.
 template <typename E> constexpr int PIECE = 16 / (int)sizeof(E);
-// k of one tile: 128 bytes of it.
-template <typename E> constexpr int DEPTH = 128 / (int)sizeof(E);
+// k of one stage of a tile: 64 bytes of it, as much as the matrix instructions
+// take of a lane's piece.
+template <typename E> constexpr int DEPTH = 64 / (int)sizeof(E);
 
 // Reads as zeros wherever a piece lies past the operand's end.
 __device__ const u4 nothing = {0, 0, 0, 0};
@@ -45,17 +46,26 @@ DEV_INLINE f4 mul(float, u4 a, u4 b, f4 c) {
     return c;
 }
 
-// 16 bytes a lane from memory to LDS, lane l's to to[l]. The caller waits: the
-// compiler, which would know of the builtin's loads, has every transposing read
-// wait for all of them, also those of the next tile (600 us in place of 440 for
-// 8192 x 2048 x 16384).
-DEV_INLINE void load_to_lds(const void* p, u4* to) {
+// 16 bytes a lane from memory to LDS, lane l's to to[l]: from a wave's address
+// and a lane's offset, or from a lane's address. The caller waits: the compiler,
+// which would know of the builtin's loads, has every transposing read wait for
+// all of them, also those of the stages to come (600 us in place of 440 for
+// 8192 x 2048 x 16384). The reads of LDS keep their distance by wait_and_meet,
+// which no memory access and no other asm crosses.
+DEV_INLINE void load_to_lds(const void* base, unsigned bytes, unsigned to) {
 #ifdef __HIP_DEVICE_COMPILE__
-    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_PTR(u4))to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(to), "v"(bytes), "s"((__attribute__((address_space(1))) const void*)base)
+                 : "m0");
+#endif
+}
+DEV_INLINE void load_to_lds(const void* p, unsigned to) {
+#ifdef __HIP_DEVICE_COMPILE__
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
-                 : "s"(at), "v"((__attribute__((address_space(1))) const void*)p)
-                 : "memory", "m0");
+                 : "s"(to), "v"((__attribute__((address_space(1))) const void*)p)
+                 : "m0");
 #endif
 }
 
@@ -63,122 +73,132 @@ DEV_INLINE void load_to_lds(const void* p, u4* to) {
 // columns), or the result's index together (rows of it are k).
 enum class Lie { K, INDEX };
 
-// One operand's tile of SPAN indexes by DEPTH k, in LDS as the operand lies in
-// memory, its pieces permuted so that the lanes that read together meet
-// different banks: by the low bits of the row's place in its fragment where k
-// lies together; else by the 8 rows of k (bf16, pairs of pieces) or the 4 (fp32,
+// One operand's stages of SPAN indexes by DEPTH k, in LDS as the operand lies in
+// memory, the pieces permuted so that the lanes that read together meet
+// different banks: by the place of the row in its fragment where k lies
+// together; else by the 8 rows of k (bf16, pairs of pieces) or the 4 (fp32,
 // fours of pieces) that one cycle of 64 banks takes values of.
 // JUMP: a fragment's 16 indexes are four runs of 4, 4 * JUMP apart; JUMP of
 // them, 4 apart, cover 16 * JUMP indexes, and a lane's accumulators 4 * JUMP
 // neighbours of the result, which it stores in one piece.
 template <typename E, Lie LIE, int SPAN, int THREADS, bool DIRECT, int JUMP>
 struct Operand {
-    static constexpr int P = PIECE<E>, PIECES = SPAN * 8;
-    static constexpr int ROUNDS = (PIECES + THREADS - 1) / THREADS;
-    static constexpr int ROW = LIE == Lie::K ? 8 : SPAN / P;  // pieces of a row in LDS
+    static constexpr int P = PIECE<E>, PIECES = SPAN * 4;
+    // Every thread takes part in every round, so that each wave has as many loads
+    // under way: ROOM pieces of a stage, the last ones without use.
+    static constexpr int ROUNDS = (PIECES + THREADS - 1) / THREADS, ROOM = ROUNDS * THREADS;
+    static constexpr int ROW = LIE == Lie::K ? 4 : SPAN / P;  // pieces of a row in LDS
     static constexpr int KEPT = (ROW & -ROW) - 1;  // bits that may turn without leaving it
-    static_assert(PIECES % 64 == 0, "a wave stages in a round or does not");
 
-    const E* at[ROUNDS];  // this thread's pieces of the tile at k = 0
-    int have[ROUNDS];     // elements of it along the index (INDEX), 0 or less: none
+    const E* base;        // the tile's first index and k
+    int64_t pitch;
+    int inside;           // indexes of the tile that exist, K: 1 at least
+    int half, other;      // K: indexes from `half` on lie `other` rows further
+    unsigned at[ROUNDS];  // this thread's pieces: elements from base on, at k = 0
     u4 held[DIRECT ? 1 : ROUNDS];
 
     static DEV_INLINE int swizzle(int row, int piece) {
-        return LIE == Lie::K    ? piece ^ ((row & 3) | (row / (4 * JUMP) & 1) << 2)
+        const int run = row / (4 * JUMP);
+        return LIE == Lie::K    ? piece ^ ((run & 1) << 1 | (run >> 1 & 1))
                : sizeof(E) == 2 ? piece ^ (((row & 3) | (row >> 1 & 4)) << 1 & KEPT)
                                 : piece ^ ((row >> 2 & 3) << 2 & KEPT);
     }
 
-    // Whether this wave has pieces in a round; in all but the last every one has.
-    static DEV_INLINE bool stages(int r) {
-        return (r + 1) * THREADS <= PIECES ||
-               r * THREADS + (int)__builtin_amdgcn_readfirstlane(threadIdx.x) < PIECES;
+    // A thread's row of the stage in LDS, and its piece of that row in memory.
+    static DEV_INLINE int row_of(int r) { return (r * THREADS + (int)threadIdx.x) % PIECES / ROW; }
+    static DEV_INLINE int piece_of(int r) {
+        return swizzle(row_of(r), (r * THREADS + (int)threadIdx.x) % PIECES % ROW);
     }
 
-    // `index(i)`: the operand's index for the tile's i-th, inside of it always
-    // (K) or the first of a run (INDEX); `count`: how many indexes there are.
-    template <typename F>
-    DEV_INLINE void start(const E* base, int64_t pitch, int count, F&& index) {
+    // From the index `first` on, `count` of them in all. From the tile's `half` on
+    // K's indexes are those of its first half, `other` rows further. Indexes past
+    // the end read the last ones: nothing of theirs is stored.
+    DEV_INLINE void start(const E* p, int64_t pitch_, int first, int count, int half, int other) {
+        pitch = pitch_;
+        base = p + (LIE == Lie::K ? first * pitch : first);
+        inside = count - first;
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
-            const int slot = r * THREADS + threadIdx.x, row = slot / ROW;
-            const int piece = swizzle(row, slot % ROW);
+            const int row = row_of(r);
             if constexpr (LIE == Lie::K) {
-                at[r] = base + index(row) * pitch + piece * P;
-                have[r] = piece * P;  // its k
+                int i = row % half;
+                if (i >= inside) i = inside - 1;
+                at[r] = (unsigned)((i + (row >= half ? (int64_t)other : 0)) * pitch) + piece_of(r) * P;
             } else {
-                const int64_t i = index(piece * P);
-                at[r] = base + row * pitch + i;
-                have[r] = i < count ? (int)(count - i < P ? count - i : P) : 0;
+                const int i = piece_of(r) * P;
+                at[r] = (unsigned)(row * pitch) + (DIRECT && i >= inside ? inside - P : i);
             }
         }
     }
 
-    // Elements of a piece that exist in the tile at k0.
+    // Elements of a piece that exist in the stage at k0.
     DEV_INLINE int left(int r, int k0, int k_hi) const {
-        if constexpr (LIE == Lie::K) return k_hi - k0 - have[r];
-        else return k0 + (r * THREADS + (int)threadIdx.x) / ROW < k_hi ? have[r] : 0;
+        if constexpr (LIE == Lie::K) return k_hi - k0 - piece_of(r) * P;
+        else return k0 + row_of(r) >= k_hi ? 0 : DIRECT ? P : inside - piece_of(r) * P;
     }
 
-    DEV_INLINE void fetch(u4* tile, int64_t pitch, int k0, int k_hi) {
-        const int64_t step = LIE == Lie::K ? k0 : (int64_t)k0 * pitch;
-        const bool whole = k0 + DEPTH<E> <= k_hi;
+    // Every piece of the stage exists: unaligned ones may end with the indexes.
+    DEV_INLINE bool whole(int k0, int k_hi) const {
+        return k0 + DEPTH<E> <= k_hi && (LIE == Lie::K || DIRECT || SPAN <= inside);
+    }
+
+    // One round of a whole stage.
+    DEV_INLINE void fetch_round(int r, unsigned stage, int k0) const {
+        const unsigned to = stage + __builtin_amdgcn_readfirstlane(threadIdx.x) * 16;
+        load_to_lds(base + (LIE == Lie::K ? k0 : k0 * pitch), at[r] * (unsigned)sizeof(E),
+                    to + r * THREADS * 16);
+    }
+
+    DEV_INLINE void fetch(unsigned stage, int k0, int k_hi) {
+        const E* p = base + (LIE == Lie::K ? k0 : k0 * pitch);
+        const bool whole = this->whole(k0, k_hi);
+        const unsigned to = stage + __builtin_amdgcn_readfirstlane(threadIdx.x) * 16;
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
-            if (!stages(r)) continue;
-            const E* p = at[r] + step;
+            const int n = whole ? P : left(r, k0, k_hi);
             if constexpr (DIRECT) {
                 // aligned pitches: a piece exists whole or not at all
-                if (LIE == Lie::INDEX || !whole)
-                    if (left(r, k0, k_hi) <= 0) p = reinterpret_cast<const E*>(&nothing);
-                u4* to = tile + r * THREADS + (threadIdx.x & ~63);
-                load_to_lds(p, to);
+                load_to_lds(n > 0 ? (const void*)(p + at[r]) : &nothing, to + r * THREADS * 16);
             } else {
                 E v[P];
-                const int n = LIE == Lie::K && whole ? P : left(r, k0, k_hi);
-                load_run<E, P>(p, n, v);
+                load_run<E, P>(p + at[r], n, v);
                 held[r] = __builtin_bit_cast(u4, v);
             }
         }
     }
 
-    DEV_INLINE void settle(u4* tile) const {
+    DEV_INLINE void settle(u4* stage) const {
         if constexpr (!DIRECT)
 #pragma unroll
-            for (int r = 0; r < ROUNDS; ++r)
-                if (stages(r)) tile[r * THREADS + threadIdx.x] = held[r];
+            for (int r = 0; r < ROUNDS; ++r) stage[r * THREADS + threadIdx.x] = held[r];
     }
 
     // The piece of the matrix instructions for the 16 indexes of the fragment that
-    // starts at `first`, at the tile's k from `k` pieces of four groups on.
-    static DEV_INLINE u4 read(const u4* tile, int first, int k) {
+    // starts at `first`.
+    static DEV_INLINE u4 read(const u4* stage, int first) {
         const int lane = threadIdx.x & 63, group = lane >> 4;
         if constexpr (LIE == Lie::K) {
             const int row = first + (lane >> 2 & 3) * 4 * JUMP + (lane & 3);
-            return tile[row * 8 + swizzle(row, k * 4 + group)];
+            return stage[row * 4 + swizzle(row, group)];
         } else if constexpr (sizeof(E) == 2) {
             // 16 lanes read 4 k by 16 indexes, 8 bytes each, and get back the 4 k
             // of one index each
-            u4 out;
+            s4 v[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = k * 32 + group * 8 + h * 4 + ((lane & 15) >> 2);
+                const int row = group * 8 + h * 4 + ((lane & 15) >> 2);
                 const int i = first + (lane & 3) * 4;
-                const char* p = (const char*)(tile + row * ROW + swizzle(row, i / P)) + (i % P) * 2;
-                const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s4))p);
-                out[2 * h] = __builtin_bit_cast(u4, (__attribute__((ext_vector_type(8))) short){
-                    v[0], v[1], v[2], v[3], 0, 0, 0, 0})[0];
-                out[2 * h + 1] = __builtin_bit_cast(u4, (__attribute__((ext_vector_type(8))) short){
-                    v[0], v[1], v[2], v[3], 0, 0, 0, 0})[1];
+                const char* p = (const char*)(stage + row * ROW + swizzle(row, i / P)) + (i % P) * 2;
+                v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s4))p);
             }
-            return out;
+            return __builtin_bit_cast(u4, v);
         } else {
             const int i = first + (lane & 15);
             u4 out;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const int row = k * 16 + group * 4 + s;
-                out[s] = reinterpret_cast<const unsigned*>(tile + row * ROW + swizzle(row, i / P))[i % P];
+                const int row = group * 4 + s;
+                out[s] = reinterpret_cast<const unsigned*>(stage + row * ROW + swizzle(row, i / P))[i % P];
             }
             return out;
         }
@@ -214,9 +234,12 @@ DEV_INLINE void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
     tn = in / rows;
 }
 
-template <int BM_, int BN_, int WM_, int WN_>
+// BM x BN of a result by WM x WN waves, with STAGES of the operands in LDS.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_ = 4>
 struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
+    static constexpr int STAGES = STAGES_;
+    static_assert(STAGES == 4 || STAGES == 5, "the waits count one or two stages under way");
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
     static_assert(MI * WM * 16 == BM && NI * WN * 16 == BN, "whole fragments");
 };
@@ -288,7 +311,6 @@ DEV_INLINE void finish(const Args<E>& p, const f4 (&acc)[T::MI][T::NI], int tm, 
         }
         if (END == End::GATED_GRAD && p.part) {
             float* sums = reinterpret_cast<float*>(lds);  // [WM][2][HALF]
-            __syncthreads();  // the tiles in LDS have been read
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const float a = row_sum16(sg[c]), b = row_sum16(su[c]);
@@ -332,25 +354,14 @@ DEV_INLINE void finish(const Args<E>& p, const f4 (&acc)[T::MI][T::NI], int tm, 
     }
 }
 
-// The order of a tile's instructions: the first half's fragments are read, then
-// the second half's between the first half's products.
-template <typename E, Lie LA, Lie LB, typename T>
-DEV_INLINE void interleave() {
-#ifdef __HIP_DEVICE_COMPILE__
-    // LDS instructions a fragment, products a fragment pair
-    constexpr int RA = LA == Lie::K ? 1 : sizeof(E) == 2 ? 2 : 4;
-    constexpr int RB = LB == Lie::K ? 1 : sizeof(E) == 2 ? 2 : 4;
-    constexpr int READS = T::MI * RA + T::NI * RB;
-    constexpr int PRODUCTS = T::MI * T::NI * (sizeof(E) == 2 ? 1 : 4);
-    constexpr int EACH = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
-    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-#pragma unroll
-    for (int r = 0; r < READS; ++r) {
-        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2 * PRODUCTS - EACH * READS, 0);
-#endif
+// Waits until at most `loads` of this wave's loads and none of its LDS reads are
+// under way, then for the other waves.
+template <int LOADS>
+DEV_INLINE void wait_and_meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((LOADS & 15) | (LOADS >> 4) << 14 | 7 << 4);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 template <typename E, typename T, Lie LA, Lie LB, End END, bool DIRECT>
@@ -358,9 +369,12 @@ __global__ void __launch_bounds__(T::THREADS)
 product_kernel(Args<E> p) {
     constexpr bool GATED = END == End::GATED || END == End::GATED_GRAD;
     constexpr int HALF = T::BN / 2, COLS = GATED ? HALF : T::BN;  // of the result a block
-    constexpr int PIECES = (T::BM + T::BN) * 8, BD = DEPTH<E>;
-    __shared__ u4 lds[2][PIECES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int NB = GATED ? T::NI / 2 : T::NI;  // a wave's fragments side by side
+    constexpr int BD = DEPTH<E>;
+    using A = Operand<E, LA, T::BM, T::THREADS, DIRECT, 1>;
+    using B = Operand<E, LB, T::BN, T::THREADS, DIRECT, GATED ? NB : 1>;
+    __shared__ u4 lds[T::STAGES][A::ROOM + B::ROOM];
+    const int wave = threadIdx.x >> 6;
     const int wm = wave / T::WN, wn = wave % T::WN;
     int tm, tn;
     tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
@@ -368,64 +382,118 @@ product_kernel(Args<E> p) {
     const int k_lo = blockIdx.z * p.per_split;
     const int k_hi = k_lo + p.per_split < p.K ? k_lo + p.per_split : p.K;
 
-    constexpr int NB = GATED ? T::NI / 2 : T::NI;  // a wave's fragments side by side
-    Operand<E, LA, T::BM, T::THREADS, DIRECT, 1> a;
-    Operand<E, LB, T::BN, T::THREADS, DIRECT, GATED ? NB : 1> b;
-    a.start(p.a, p.pitch_a, p.M, [&](int i) {
-        const int m = m0 + i;  // rows past the end read the last one: none is stored
-        return (int64_t)(LA == Lie::K && m >= p.M ? p.M - 1 : m);
-    });
-    b.start(p.b, p.pitch_b, p.N, [&](int i) {
-        const int n = n0 + (GATED ? i % HALF : i);
-        const int in = LB == Lie::K && n >= p.N ? p.N - 1 : n;
-        return (int64_t)in + (GATED && i >= HALF ? p.N : 0);
-    });
+    A a;
+    B b;
+    a.start(p.a, p.pitch_a, m0, p.M, T::BM, 0);
+    b.start(p.b, p.pitch_b, n0, p.N, GATED ? HALF : T::BN, GATED ? p.N : 0);
+    constexpr int STAGES = T::STAGES;
+    const unsigned lds_at = (unsigned)(uintptr_t)(LDS_PTR(u4))&lds[0][0];
+    const auto fetch = [&](int place, int k0) {
+        const unsigned to = lds_at + place * (A::ROOM + B::ROOM) * 16;
+        a.fetch(to, k0, k_hi);
+        b.fetch(to + A::ROOM * 16, k0, k_hi);
+    };
+    const auto settle = [&](int place) {
+        a.settle(lds[place]);
+        b.settle(lds[place] + A::ROOM);
+    };
+    // Fragments in registers: those of b of two stages, of a the next AHEAD + 1.
+    constexpr int RING = T::MI < 4 ? T::MI : 2 * T::MI % 4 == 0 ? 4 : 5, AHEAD = RING - 1;
+    static_assert(2 * T::MI % RING == 0, "a turn of the loop ends where it began");
+    static_assert(T::NI <= T::MI, "b's fragments are read beside a's");
+    u4 af[RING], bf[2][T::NI];
+    const auto read_b = [&](int set, int j, int place) {
+        // gated: the wave's first half of columns are gates, then their values
+        const int first = GATED ? (j / NB) * HALF + wn * NB * 16 + j % NB * 4
+                                : (wn * NB + j) * 16;
+        bf[set][j] = B::read(lds[place] + A::ROOM, first);
+    };
+    const auto read_a = [&](int slot, int i, int place) {
+        af[slot] = A::read(lds[place], (wm * T::MI + i) * 16);
+    };
+    // LDS instructions of a fragment, matrix instructions of a product.
+    constexpr int RA = LA == Lie::K ? 1 : sizeof(E) == 2 ? 2 : 4;
+    constexpr int RB = LB == Lie::K ? 1 : sizeof(E) == 2 ? 2 : 4;
+    constexpr int EACH = sizeof(E) == 2 ? 1 : 4;
 
     f4 acc[T::MI][T::NI] = {};
-    int turn = 0;
+    // Stage t lies in place t % STAGES. While its products run, row of fragments by
+    // row, its last fragments and its successor's first are read: the successor has
+    // landed when the waves meet at its beginning, and the place of the stage
+    // before it is free for the one STAGES - 1 on.
+    constexpr int LOADS = DIRECT ? A::ROUNDS + B::ROUNDS : 0;
     if (k_lo < k_hi) {
-        a.fetch(lds[0], p.pitch_a, k_lo, k_hi);
-        b.fetch(lds[0] + T::BM * 8, p.pitch_b, k_lo, k_hi);
-        a.settle(lds[0]);
-        b.settle(lds[0] + T::BM * 8);
-    }
-    for (int k0 = k_lo; k0 < k_hi; k0 += BD) {
-        // this tile has landed, and everyone is done with the other buffer
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        const u4* now = lds[turn];
-        u4* next = lds[turn ^ 1];
-        const bool more = k0 + BD < k_hi;
-        if (more) {
-            a.fetch(next, p.pitch_a, k0 + BD, k_hi);
-            b.fetch(next + T::BM * 8, p.pitch_b, k0 + BD, k_hi);
-        }
-        u4 af[2][T::MI], bf[2][T::NI];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-#pragma unroll
-            for (int j = 0; j < T::NI; ++j) {
-                // gated: the wave's first half of columns are gates, then their values
-                const int first = GATED ? (j / NB) * HALF + wn * NB * 16 + j % NB * 4
-                                        : (wn * NB + j) * 16;
-                bf[k][j] = b.read(now + T::BM * 8, first, k);
+        for (int s = 0; s < STAGES - 1; ++s)
+            if (k_lo + s * BD < k_hi) {
+                fetch(s, k_lo + s * BD);
+                if (!DIRECT && s + 1 < STAGES - 1) settle(s);
             }
+        if (DIRECT && k_lo + (STAGES - 2) * BD >= k_hi) wait_and_meet<0>();
+        else if (DIRECT) wait_and_meet<(STAGES - 2) * LOADS>();
+        else wait_and_meet<63>();
 #pragma unroll
-            for (int i = 0; i < T::MI; ++i) af[k][i] = a.read(now, (wm * T::MI + i) * 16, k);
-        }
+        for (int j = 0; j < T::NI; ++j) read_b(0, j, 0);
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-                for (int j = 0; j < T::NI; ++j) acc[i][j] = mul(E(), bf[k][j], af[k][i], acc[i][j]);
-        interleave<E, LA, LB, T>();
-        if (more) {
-            a.settle(next);
-            b.settle(next + T::BM * 8);
-        }
-        turn ^= 1;
+        for (int i = 0; i < AHEAD; ++i) read_a(i, i, 0);
     }
+    int place = 0;  // of the stage whose products run
+    // Two stages from k0 on. SPREAD: all that they wait for and fetch exists whole,
+    // and is fetched a round at a time between the products: all at once the loads
+    // hold up the waves until the memory has taken them.
+    const auto two_stages = [&](int k0, auto spread) {
+        constexpr bool SPREAD = decltype(spread)::value;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int at = k0 + s * BD, far = at + (STAGES - 1) * BD;
+            if (!SPREAD && at >= k_hi) break;
+            const int after = place + 1 < STAGES ? place + 1 : 0;
+            const int before = place > 0 ? place - 1 : STAGES - 1;
+            const unsigned to = lds_at + before * (A::ROOM + B::ROOM) * 16;
+            if constexpr (!DIRECT) {
+                if (far - BD < k_hi) settle(before > 0 ? before - 1 : STAGES - 1);
+                wait_and_meet<63>();
+            } else if (SPREAD || far - BD < k_hi) {
+                wait_and_meet<(STAGES - 3) * LOADS>();
+            } else if (STAGES > 4 && far - 2 * BD < k_hi) {
+                wait_and_meet<LOADS>();  // of the STAGES - 3 stages that may be on their way one is
+            } else {
+                wait_and_meet<0>();
+            }
+            if (!SPREAD && far < k_hi) fetch(before, far);
+#pragma unroll
+            for (int i = 0; i < T::MI; ++i) {
+                const int now = s * T::MI + i, next = i + AHEAD;
+                read_a((now + AHEAD) % RING, next % T::MI, next < T::MI ? place : after);
+                if (i < T::NI) read_b((s + 1) & 1, i, after);
+                if constexpr (SPREAD)
+#pragma unroll
+                    for (int n = i * LOADS / T::MI; n < (i + 1) * LOADS / T::MI; ++n) {
+                        if (n < A::ROUNDS) a.fetch_round(n, to, far);
+                        else b.fetch_round(n - A::ROUNDS, to + A::ROOM * 16, far);
+                    }
+#pragma unroll
+                for (int j = 0; j < T::NI; ++j)
+                    acc[i][j] = mul(E(), bf[s & 1][j], af[now % RING], acc[i][j]);
+#ifdef __HIP_DEVICE_COMPILE__
+                __builtin_amdgcn_sched_group_barrier(0x100, RA, 0);
+                if (i < T::NI) __builtin_amdgcn_sched_group_barrier(0x100, RB, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, T::NI * EACH, 0);
+#endif
+            }
+            place = after;
+        }
+    };
+    int k0 = k_lo;
+    if constexpr (DIRECT) {
+        // as long as the second of the two fetches a whole stage
+        const int last = a.whole(k_lo, k_hi) && b.whole(k_lo, k_hi) ? k_hi - (STAGES + 1) * BD : k_lo - 1;
+#pragma unroll 1
+        for (; k0 <= last; k0 += 2 * BD) two_stages(k0, std::true_type());
+    }
+#pragma unroll 1
+    for (; k0 < k_hi; k0 += 2 * BD) two_stages(k0, std::false_type());
+    wait_and_meet<0>();  // nothing is on its way into LDS any more
 
     // Fragment j's accumulator holds row lane % 16 and, as its element q, column
     // (lane / 16) * 4 * JUMP + 4 j + q. Tiles inside the result are stored
@@ -473,15 +541,15 @@ struct Rate {
 template <typename E, typename F>
 void each_tile(F&& f) {
     if constexpr (sizeof(E) == 2) {
-        f(Tile<256, 256, 2, 4>(), Rate{1, 4.9, 0});
+        f(Tile<256, 256, 2, 4, 5>(), Rate{1, 4.9, 0});
         f(Tile<192, 256, 2, 4>(), Rate{1, 4.7, 0});
         f(Tile<160, 256, 2, 4>(), Rate{1, 4.5, 0});
         f(Tile<128, 256, 2, 4>(), Rate{1, 4.3, 0});
-        f(Tile<128, 128, 2, 2>(), Rate{2, 3.5, 0.8});
-        f(Tile<64, 64, 2, 2>(), Rate{4, 2.0, 0.5});
+        f(Tile<128, 128, 2, 2>(), Rate{2, 3.5, 0.4});
+        f(Tile<64, 64, 2, 2>(), Rate{4, 2.0, 0.25});
     } else {
-        f(Tile<128, 128, 2, 2>(), Rate{2, 0.5, 2.2});
-        f(Tile<64, 64, 2, 2>(), Rate{4, 0.47, 0.75});
+        f(Tile<128, 128, 2, 2>(), Rate{2, 0.5, 1.1});
+        f(Tile<64, 64, 2, 2>(), Rate{4, 0.47, 0.38});
     }
 }
 
