@@ -2,15 +2,18 @@
 // (K9-K11): checks, outputs and workspaces; the kernels sit behind extern "C"
 // launchers as in bindings.cpp.
 //
-// Each operator is one call: checks, the autograd node (in C++: a Python one
-// costs a training step of a small batch several times its kernels) and the
-// launches. It runs on its first argument's device and that device's current
-// stream. Workspaces are allocated per call on that stream, so calls on several
-// streams and captured graphs share none.
+// Each operator is one call: checks, launches and its autograd node, in C++ and
+// of plain members: a small batch's training step is bound by the host, 62 us
+// with torch's custom functions and their maps of saved values, 56 with these
+// nodes, 44 for a bare product by two. It runs on its first argument's device and
+// that device's current stream. Workspaces are allocated per call on that stream,
+// so calls on several streams and captured graphs share none.
 
 #include <torch/extension.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -46,7 +49,8 @@ namespace {
 
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 constexpr int64_t MOST = std::numeric_limits<int>::max() / 2;
@@ -108,6 +112,21 @@ bool tracked(const T&... t) {
     return any;
 }
 
+// What the nodes below share: the lock that a node holds while it runs, saved
+// tensors, and the edges to the inputs.
+template <typename N, typename... T>
+std::shared_ptr<N> node_of(const T&... inputs) {
+    std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+    return node;
+}
+
+SavedVariable save(const OptTensor& t) { return SavedVariable(t ? *t : Tensor(), false); }
+OptTensor optional(const SavedVariable& s) {
+    Tensor t = s.unpack();
+    return t.defined() ? OptTensor(t) : OptTensor();
+}
+
 // The kernels' gradients are not differentiable themselves: asked for with
 // create_graph, they raise when someone differentiates them, and are no constants.
 variable_list once(variable_list grads, const char* name) {
@@ -157,27 +176,27 @@ std::tuple<Tensor, Tensor> layer_norm_bwd(const Tensor& x, const OptTensor& resi
     return {dx, dwb};
 }
 
-struct LayerNorm : torch::autograd::Function<LayerNorm> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
-                                 const OptTensor& bias, const OptTensor& residual, double eps) {
-        auto [y, s] = layer_norm_fwd(x, weight, bias, residual, eps);
-        ctx->set_materialize_grads(false);
-        ctx->saved_data["eps"] = eps;
-        ctx->saved_data["bias"] = bias.has_value();
-        ctx->save_for_backward({x, weight, residual ? *residual : Tensor()});
-        return residual ? variable_list{y, s} : variable_list{y};
+struct LayerNormBackward : Node {
+    SavedVariable x, weight, residual;
+    double eps;
+    std::string name() const override { return "LayerNormBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        x.reset_data();
+        weight.reset_data();
+        residual.reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &residual = saved[2];
-        const bool fused = residual.defined();
-        const Tensor dy = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(x);
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        const Tensor in = x.unpack();
+        const OptTensor res = optional(residual);
+        const Tensor dy = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(in);
         OptTensor ds;
-        if (fused && grads[1].defined()) ds = grads[1].contiguous();
-        auto [dx, dwb] = layer_norm_bwd(x, fused ? OptTensor(residual) : OptTensor(), saved[1], dy,
-                                        ds, ctx->saved_data["eps"].toDouble());
-        return once({dx, dwb[0], ctx->saved_data["bias"].toBool() ? dwb[1] : Tensor(),
-                     fused ? dx : Tensor(), Tensor()}, "layer_norm");
+        if (res && grads[1].defined()) ds = grads[1].contiguous();
+        auto [dx, dwb] = layer_norm_bwd(in, res, weight.unpack(), dy, ds, eps);
+        return once({dx, should_compute_output(1) ? dwb[0] : Tensor(),
+                     should_compute_output(2) ? dwb[1] : Tensor(), res ? dx : Tensor()},
+                    "layer_norm");
     }
 };
 
@@ -191,11 +210,19 @@ variable_list layer_norm(const Tensor& x, const Tensor& weight, const OptTensor&
     check(weight, "weight", x, x.scalar_type(), {dim});
     if (bias) check(*bias, "bias", x, x.scalar_type(), {dim});
     if (residual) check(*residual, "residual", x, x.scalar_type(), x.sizes());
-    if (tracked(x, weight, bias, residual))
-        return LayerNorm::apply(x.contiguous(), weight.contiguous(), contiguous(bias),
-                                contiguous(residual), eps);
-    auto [y, s] = layer_norm_fwd(x.contiguous(), weight.contiguous(), contiguous(bias),
-                                 contiguous(residual), eps);
+    const bool track = tracked(x, weight, bias, residual);
+    const Tensor in = x.contiguous(), w = weight.contiguous();
+    const OptTensor b = contiguous(bias), r = contiguous(residual);
+    auto [y, s] = layer_norm_fwd(in, w, b, r, eps);
+    if (track) {
+        auto node = node_of<LayerNormBackward>(in, w, b, r);
+        node->x = save(in);
+        node->weight = save(w);
+        node->residual = save(r);
+        node->eps = eps;
+        torch::autograd::set_history(y, node);
+        if (r) torch::autograd::set_history(s, node);
+    }
     return residual ? variable_list{y, s} : variable_list{y};
 }
 
@@ -237,27 +264,25 @@ std::tuple<Tensor, Tensor> gated_recurrence_bwd(const Tensor& gates, const Tenso
     return {dgates, dh0};
 }
 
-struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& gates, const OptTensor& h0,
-                                 const OptTensor& lengths) {
-        auto [y, hT, kept] = gated_recurrence_fwd(gates, h0, lengths, true);
-        ctx->set_materialize_grads(false);
-        ctx->saved_data["h0"] = h0.has_value();
-        ctx->save_for_backward({gates, kept, lengths ? *lengths : Tensor()});
-        return {y, hT};
+struct GatedRecurrenceBackward : Node {
+    SavedVariable gates, kept, lengths;
+    std::string name() const override { return "GatedRecurrenceBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        gates.reset_data();
+        kept.reset_data();
+        lengths.reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        const Tensor& gates = saved[0];
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        const Tensor g = gates.unpack();
         const Tensor dy = grads[0].defined()
             ? grads[0].contiguous()
-            : torch::zeros({gates.size(0), gates.size(1), gates.size(2) / 3}, gates.options());
-        OptTensor dhT, lengths;
+            : torch::zeros({g.size(0), g.size(1), g.size(2) / 3}, g.options());
+        OptTensor dhT;
         if (grads[1].defined()) dhT = grads[1].contiguous();
-        if (saved[2].defined()) lengths = saved[2];
-        auto [dgates, dh0] = gated_recurrence_bwd(gates, saved[1], lengths, dy, dhT);
-        return once({dgates, ctx->saved_data["h0"].toBool() ? dh0 : Tensor(), Tensor()},
-                    "gated_recurrence");
+        auto [dgates, dh0] = gated_recurrence_bwd(g, kept.unpack(), optional(lengths), dy, dhT);
+        return once({dgates, should_compute_output(1) ? dh0 : Tensor()}, "gated_recurrence");
     }
 };
 
@@ -272,12 +297,18 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const OptTensor
                 "gates is too large");
     if (h0) check(*h0, "h0 (the state is not rounded)", gates, torch::kFloat32, {B, H});
     if (lengths) check(*lengths, "lengths", gates, torch::kInt32, {B});
-    if (tracked(gates, h0)) {
-        auto out = GatedRecurrence::apply(gates.contiguous(), contiguous(h0), contiguous(lengths));
-        return {out[0], out[1]};
+    const bool track = tracked(gates, h0);
+    const Tensor g = gates.contiguous();
+    const OptTensor h = contiguous(h0), n = contiguous(lengths);
+    auto [y, hT, kept] = gated_recurrence_fwd(g, h, n, track);
+    if (track) {
+        auto node = node_of<GatedRecurrenceBackward>(g, h);
+        node->gates = save(g);
+        node->kept = save(kept);
+        node->lengths = save(n);
+        torch::autograd::set_history(y, node);
+        torch::autograd::set_history(hT, node);
     }
-    auto [y, hT, kept] =
-        gated_recurrence_fwd(gates.contiguous(), contiguous(h0), contiguous(lengths), false);
     return {y, hT};
 }
 
@@ -328,19 +359,22 @@ variable_list gated_linear_bwd(const Tensor& x, const Tensor& weight, const OptT
     return {dx, dw, db};
 }
 
-struct GatedLinear : torch::autograd::Function<GatedLinear> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
-                                 const OptTensor& bias) {
-        ctx->save_for_backward({x, weight, bias ? *bias : Tensor()});
-        return {gated_linear_fwd(x, weight, bias)};
+struct GatedLinearBackward : Node {
+    SavedVariable x, weight, bias;
+    std::string name() const override { return "GatedLinearBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        x.reset_data();
+        weight.reset_data();
+        bias.reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        OptTensor bias;
-        if (saved[2].defined()) bias = saved[2];
-        return once(gated_linear_bwd(saved[0], saved[1], bias, grads[0].contiguous(),
-                                     ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-                                     bias && ctx->needs_input_grad(2)), "gated_linear");
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        return once(gated_linear_bwd(x.unpack(), weight.unpack(), optional(bias),
+                                     grads[0].contiguous(), should_compute_output(0),
+                                     should_compute_output(1), should_compute_output(2)),
+                    "gated_linear");
     }
 };
 
@@ -361,9 +395,18 @@ Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
     // a tile's places are counted in 32 bits from its first: 256 rows, or a gate's
     // row and its value's
     TORCH_CHECK((F + 256) * K <= MOST && 512 * F <= MOST, "weight is too large");
-    if (tracked(x, weight, bias))
-        return GatedLinear::apply(x.contiguous(), weight.contiguous(), contiguous(bias))[0];
-    return gated_linear_fwd(x.contiguous(), weight.contiguous(), contiguous(bias));
+    const bool track = tracked(x, weight, bias);
+    const Tensor in = x.contiguous(), w = weight.contiguous();
+    const OptTensor b = contiguous(bias);
+    auto y = gated_linear_fwd(in, w, b);
+    if (track) {
+        auto node = node_of<GatedLinearBackward>(in, w, b);
+        node->x = save(in);
+        node->weight = save(w);
+        node->bias = save(b);
+        torch::autograd::set_history(y, node);
+    }
+    return y;
 }
 
 }  // namespace
