@@ -277,13 +277,22 @@ DEV_INLINE void finish(const Args<E>& p, const f4 (&acc)[T::MI][T::NI], int tm, 
                 bu[c] = to_f(u[c]);
             }
         }
-        E d[C];
+        // dy of all rows is on its way before the first is used
+        E d[END == End::GATED_GRAD ? T::MI : 1][C];
+        if (END == End::GATED_GRAD) {
+#pragma unroll
+            for (int i = 0; i < T::MI; ++i) {
+                const int row = row0 + i * 16;
+                load_piece<E, C, INSIDE>(p.dy + (int64_t)row * p.N + col, row < p.M ? have : 0, d[i]);
+            }
+#ifdef __HIP_DEVICE_COMPILE__
+            __builtin_amdgcn_sched_barrier(0);
+#endif
+        }
 #pragma unroll
         for (int i = 0; i < T::MI; ++i) {
             const int row = row0 + i * 16;
             if (!INSIDE && (row >= p.M || have <= 0)) continue;
-            if (END == End::GATED_GRAD)
-                load_piece<E, C, INSIDE>(p.dy + (int64_t)row * p.N + col, have, d);
             E out[C], out2[C];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -294,7 +303,7 @@ DEV_INLINE void finish(const Args<E>& p, const f4 (&acc)[T::MI][T::NI], int tm, 
                 if (END == End::GATED) {
                     out[c] = from_f<E>(val * u);
                 } else {
-                    const float dg = to_f(d[c]) * u * grad, du = to_f(d[c]) * val;
+                    const float dg = to_f(d[i][c]) * u * grad, du = to_f(d[i][c]) * val;
                     out[c] = from_f<E>(dg);
                     out2[c] = from_f<E>(du);
                     sg[c] += dg;
