@@ -131,18 +131,18 @@ def recurrence_oracle(gates, h0, lengths, dy, dhT):
 
 
 # ----------------------------------------------------------- gated linear unit
-def linear_oracle(x, w, b, dy):
-    """[(exact, bound)] for y, dx, dw, db (db where b is given)."""
+def linear_oracle(x, w, b, dy, device="cpu"):
+    """[(exact, bound)] for y, dx, dw, db (db where b is given), computed on `device`."""
     dt = x.dtype
     h = half(dt)
     K, F = x.shape[-1], w.shape[0] // 2
     shape = x.shape
     M = shape[:-1].numel()
-    x, w = x.detach().double().cpu().reshape(M, K), w.detach().double().cpu()
-    dy = dy.double().cpu().reshape(M, F)
+    x, w = x.detach().to(device).double().reshape(M, K), w.detach().to(device).double()
+    dy = dy.to(device).double().reshape(M, F)
     p, ep = x @ w.t(), (K + 4) * U * (x.abs() @ w.abs().t())
     if b is not None:
-        bias = b.detach().double().cpu()
+        bias = b.detach().to(device).double()
         p, ep = p + bias, ep + 2 * U * (bias.abs() + p.abs())
     g, u = p[:, :F], p[:, F:]
     eg, eu = ep[:, :F], ep[:, F:]
@@ -163,7 +163,7 @@ def linear_oracle(x, w, b, dy):
            (dx.reshape(shape), edx.reshape(shape)), (dw, edw)]
     if b is not None:
         res.append((dp.sum(0), edb.sum(0) + h * dp.sum(0).abs()))
-    return res
+    return [(exact.cpu(), bound.cpu()) for exact, bound in res]
 
 
 # Smallest step of fp32 and bf16 alike: results below it flush to zero.

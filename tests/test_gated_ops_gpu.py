@@ -233,7 +233,7 @@ def test_recurrence_offsets_past_32_bits():
 
 
 # ----------------------------------------------------------- gated linear unit
-def run_linear(M, K, F, dtype, bias=True, seed=0, shape=None):
+def run_linear(M, K, F, dtype, bias=True, seed=0, shape=None, oracle_on="cpu"):
     x = rand(M, K, seed=seed, dtype=dtype).reshape(shape or (M, K))
     w = rand(2 * F, K, seed=seed + 1, dtype=dtype, scale=max(K, 1) ** -0.5)
     b = rand(2 * F, seed=seed + 2, dtype=dtype, scale=0.3) if bias else None
@@ -241,7 +241,7 @@ def run_linear(M, K, F, dtype, bias=True, seed=0, shape=None):
     ins = leaves(x, w, b)
     y = gated_linear(x, w, b)
     got = [y] + list(torch.autograd.grad([y], ins, [dy]))
-    want = linear_oracle(x, w, b, dy)
+    want = linear_oracle(x, w, b, dy, device=oracle_on)
     check_all(got, want)
     for g, (exact, _) in zip(got, want):
         # Errors of independent signs: the result's own rounding, and dp's, whose
@@ -277,6 +277,17 @@ def test_linear_widths(K, F, dtype):
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_linear_larger(M, K, F, dtype):
     run_linear(M, K, F, dtype, seed=M)
+
+
+# every tile that the four products are cut into, whole and past its edges, with
+# and without splits, in 16-byte pieces and element by element
+@pytest.mark.parametrize("M, K, F", [
+    (4096, 2048, 4096), (5000, 1048, 2056), (5001, 1043, 2055), (8200, 1032, 2056), (8201, 1029, 2054),
+    (10240, 1024, 2048), (16384, 520, 136), (16380, 517, 129), (1500, 136, 2048), (1501, 203, 2045),
+    (300, 1024, 2048), (4090, 67, 2041), (20480, 67, 1024), (4096, 1024, 64)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_linear_tiles(M, K, F, dtype):
+    run_linear(M, K, F, dtype, seed=K, oracle_on="cuda")
 
 
 def test_linear_shapes_strides_and_partial_gradients():
