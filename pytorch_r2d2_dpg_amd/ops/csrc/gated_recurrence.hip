@@ -212,7 +212,7 @@ recurrence_fwd_kernel(Args<E> p) {
     Two<E> f[CHUNK], v[CHUNK], o[CHUNK];
     const auto fetch = [&](int chunk) {
         const int t0 = chunk * CHUNK;
-        const E* g = p.gates + 3 * t0 * step;
+        const E* g = p.gates + t0 * step * 3;
 #pragma unroll
         for (int k = 0; k < CHUNK; ++k, g += 3 * step)
             if (t0 + k < p.T) {
@@ -311,7 +311,7 @@ recurrence_bwd_kernel(Args<E> p) {
     const auto fetch = [&](int chunk) {
         const int t0 = chunk * CHUNK;
         if (!ONLY_MAP && t0 < p.T) kept = load2<EVEN>(p.kept + chunk * step, at, second);
-        const E *g = p.gates + 3 * t0 * step, *d = p.dy + t0 * step;
+        const E *g = p.gates + t0 * step * 3, *d = p.dy + t0 * step;
 #pragma unroll
         for (int k = 0; k < CHUNK; ++k, g += 3 * step, d += step)
             if (t0 + k < p.T) {
@@ -329,7 +329,7 @@ recurrence_bwd_kernel(Args<E> p) {
         // other follows without cancelling, in half the registers. dist is
         // h_{t-1} - v, g is dy silu(o).
         float m[CHUNK][2], dist[CHUNK][2], g[CHUNK][2], h[2] = {kept[0], kept[1]};
-        E* to = p.dgates + 3 * t0 * step;
+        E* to = p.dgates + t0 * step * 3;
 #pragma unroll
         for (int k = 0; k < CHUNK; ++k, to += 3 * step)
             if (t0 + k < p.T) {
