@@ -15,8 +15,8 @@ template <> DEV_INLINE float from_f<float>(float v) { return v; }
 template <> DEV_INLINE bf16 from_f<bf16>(float v) { return f2bf(v); }
 
 // sigma(x) and sigma(-x) = 1 - sigma(x) from one exponential of -|x|: neither
-// cancels where the other is near one, and a NaN is both. The exp2 and rcp instructions are within
-// 1 ulp, the argument's rounding adds |x| * 2^-24.
+// cancels where the other is near one, and a NaN is both. The exp2 and rcp
+// instructions are within 1 ulp, the argument's rounding adds |x| * 2^-24.
 DEV_INLINE void sigmoid_pair(float x, float& pos, float& neg) {
     const float e = __builtin_amdgcn_exp2f(-fabsf(x) * 1.44269504f);
     const float big = __builtin_amdgcn_rcpf(1.0f + e);

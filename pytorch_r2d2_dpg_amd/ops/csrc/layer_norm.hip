@@ -9,6 +9,8 @@
 
 #include "gated_common.h"
 
+#include <algorithm>
+
 namespace {
 
 template <typename E> constexpr int RUN = 16 / (int)sizeof(E);  // one load of a lane
@@ -245,76 +247,80 @@ norm_bwd_kernel(const E* __restrict__ x, const E* __restrict__ res,
     }
 }
 
-// Rows shorter than a run or too long for registers: the row is read again for
-// each sum over it.
-template <typename E>
-__global__ void __launch_bounds__(1024)
+// Rows too long for registers, by 1024 threads, or shorter than a run, by a wave:
+// the row is read again for each sum over it.
+template <typename E, int TPR>
+__global__ void __launch_bounds__(TPR)
 norm_fwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
                      const E* __restrict__ w, const E* __restrict__ b,
-                     E* __restrict__ y, E* __restrict__ s_out, int dim, float eps) {
+                     E* __restrict__ y, E* __restrict__ s_out, int64_t rows, int dim,
+                     float eps) {
     __shared__ float2 lds[2][16];
     int turn = 0;
-    const int64_t row = blockIdx.x;
-    const E* xr = x + row * dim;
-    const E* rr = res ? res + row * dim : nullptr;
-    float sum = 0.0f;
-    for (int c = threadIdx.x; c < dim; c += 1024) {
-        const float v = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
-        if (rr) s_out[row * dim + c] = from_f<E>(v);
-        sum += v;
-    }
-    float sq = 0.0f, none = 0.0f;
-    row_sums<1024>(sum, none, lds, turn);
-    const float mean = sum / dim;
-    for (int c = threadIdx.x; c < dim; c += 1024) {
-        const float d = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean;
-        sq += d * d;
-    }
-    row_sums<1024>(sq, none, lds, turn);
-    const float rstd = 1.0f / sqrtf(sq / dim + eps);
-    for (int c = threadIdx.x; c < dim; c += 1024) {
-        const float v = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
-        y[row * dim + c] = from_f<E>((v - mean) * rstd * to_f(w[c]) +
-                                     (b ? to_f(b[c]) : 0.0f));
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const E* xr = x + row * dim;
+        const E* rr = res ? res + row * dim : nullptr;
+        float sum = 0.0f;
+        for (int c = threadIdx.x; c < dim; c += TPR) {
+            const float v = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
+            if (rr) s_out[row * dim + c] = from_f<E>(v);
+            sum += v;
+        }
+        float sq = 0.0f, none = 0.0f;
+        row_sums<TPR>(sum, none, lds, turn);
+        const float mean = sum / dim;
+        for (int c = threadIdx.x; c < dim; c += TPR) {
+            const float d = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean;
+            sq += d * d;
+        }
+        row_sums<TPR>(sq, none, lds, turn);
+        const float rstd = 1.0f / sqrtf(sq / dim + eps);
+        for (int c = threadIdx.x; c < dim; c += TPR) {
+            const float v = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
+            y[row * dim + c] = from_f<E>((v - mean) * rstd * to_f(w[c]) +
+                                         (b ? to_f(b[c]) : 0.0f));
+        }
     }
 }
 
 // The row's gradient, and its mean and rstd for the weight's, which is left to
 // norm_dw_long_kernel.
-template <typename E>
-__global__ void __launch_bounds__(1024)
+template <typename E, int TPR>
+__global__ void __launch_bounds__(TPR)
 norm_bwd_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
                      const E* __restrict__ w, float* __restrict__ stats, const E* __restrict__ dy,
-                     const E* __restrict__ ds, E* __restrict__ dx, int dim, float eps) {
+                     const E* __restrict__ ds, E* __restrict__ dx, int64_t rows, int dim,
+                     float eps) {
     __shared__ float2 lds[2][16];
     int turn = 0;
-    const int64_t row = blockIdx.x;
-    const E *xr = x + row * dim, *rr = res ? res + row * dim : nullptr, *dr = dy + row * dim;
-    float sum = 0.0f, sg = 0.0f, sq = 0.0f, sgn = 0.0f;
-    for (int c = threadIdx.x; c < dim; c += 1024) {
-        sum += to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
-        sg += to_f(dr[c]) * to_f(w[c]);
-    }
-    row_sums<1024>(sum, sg, lds, turn);
-    const float mean = sum / dim;
-    sg /= dim;
-    for (int c = threadIdx.x; c < dim; c += 1024) {
-        const float n = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean;
-        sq += n * n;
-        sgn += to_f(dr[c]) * to_f(w[c]) * n;
-    }
-    row_sums<1024>(sq, sgn, lds, turn);
-    const float rstd = 1.0f / sqrtf(sq / dim + eps);
-    sgn *= rstd / dim;
-    if (threadIdx.x == 0) {
-        stats[2 * row] = mean;
-        stats[2 * row + 1] = rstd;
-    }
-    for (int c = threadIdx.x; c < dim; c += 1024) {
-        const float g = to_f(dr[c]) * to_f(w[c]);
-        const float n = (to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean) * rstd;
-        dx[row * dim + c] = from_f<E>((g - sg - n * sgn) * rstd +
-                                      (ds ? to_f(ds[row * dim + c]) : 0.0f));
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const E *xr = x + row * dim, *rr = res ? res + row * dim : nullptr, *dr = dy + row * dim;
+        float sum = 0.0f, sg = 0.0f, sq = 0.0f, sgn = 0.0f;
+        for (int c = threadIdx.x; c < dim; c += TPR) {
+            sum += to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f);
+            sg += to_f(dr[c]) * to_f(w[c]);
+        }
+        row_sums<TPR>(sum, sg, lds, turn);
+        const float mean = sum / dim;
+        sg /= dim;
+        for (int c = threadIdx.x; c < dim; c += TPR) {
+            const float n = to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean;
+            sq += n * n;
+            sgn += to_f(dr[c]) * to_f(w[c]) * n;
+        }
+        row_sums<TPR>(sq, sgn, lds, turn);
+        const float rstd = 1.0f / sqrtf(sq / dim + eps);
+        sgn *= rstd / dim;
+        if (threadIdx.x == 0) {
+            stats[2 * row] = mean;
+            stats[2 * row + 1] = rstd;
+        }
+        for (int c = threadIdx.x; c < dim; c += TPR) {
+            const float g = to_f(dr[c]) * to_f(w[c]);
+            const float n = (to_f(xr[c]) + (rr ? to_f(rr[c]) : 0.0f) - mean) * rstd;
+            dx[row * dim + c] = from_f<E>((g - sg - n * sgn) * rstd +
+                                          (ds ? to_f(ds[row * dim + c]) : 0.0f));
+        }
     }
 }
 
@@ -369,6 +375,14 @@ void with_shape(int dim, bool fused, F&& f) {
         go(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
 }
 
+template <typename E, typename F>
+void with_long(int dim, F&& f) {
+    if (dim < RUN<E>) f(std::integral_constant<int, 64>());
+    else f(std::integral_constant<int, 1024>());
+}
+// A launch has less than 2^32 threads.
+constexpr int64_t LONG_BLOCKS = 1 << 20;
+
 // Blocks of a launch: enough to fill the card several times over, and few
 // enough that each keeps its weights for several rows.
 constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 512;
@@ -384,9 +398,12 @@ int fwd(const void* x, const void* res, const void* w, const void* b, void* y,
         void* s, int64_t rows, int dim, float eps, hipStream_t st) {
     if (rows == 0) return 0;
     if (shape_of<E>(dim).threads == 0)
-        norm_fwd_long_kernel<E><<<dim3((unsigned)rows), 1024, 0, st>>>(
-            (const E*)x, (const E*)res, (const E*)w, (const E*)b, (E*)y, (E*)s,
-            dim, eps);
+        with_long<E>(dim, [&](auto t) {
+            constexpr int T = decltype(t)::value;
+            norm_fwd_long_kernel<E, T><<<(int)std::min(rows, LONG_BLOCKS), T, 0, st>>>(
+                (const E*)x, (const E*)res, (const E*)w, (const E*)b, (E*)y, (E*)s, rows, dim,
+                eps);
+        });
     else
         with_shape<E>(dim, res != nullptr, [&](auto t, auto n, auto fused) {
             constexpr int T = decltype(t)::value, N = decltype(n)::value;
@@ -405,9 +422,12 @@ int bwd(const void* x, const void* res, const void* w, const void* dy, const voi
     if (rows == 0) {
         parts = 0;
     } else if (shape_of<E>(dim).threads == 0) {
-        norm_bwd_long_kernel<E><<<dim3((unsigned)rows), 1024, 0, st>>>(
-            (const E*)x, (const E*)res, (const E*)w, stats, (const E*)dy, (const E*)ds, (E*)dx, dim,
-            eps);
+        with_long<E>(dim, [&](auto t) {
+            constexpr int T = decltype(t)::value;
+            norm_bwd_long_kernel<E, T><<<(int)std::min(rows, LONG_BLOCKS), T, 0, st>>>(
+                (const E*)x, (const E*)res, (const E*)w, stats, (const E*)dy, (const E*)ds,
+                (E*)dx, rows, dim, eps);
+        });
         LSTM_CHECK_LAUNCH();
         norm_dw_long_kernel<E><<<dim3((dim + 255) / 256, parts), 256, 0, st>>>(
             (const E*)x, (const E*)res, stats, (const E*)dy, part, rows, dim);
