@@ -54,6 +54,8 @@ using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 constexpr int64_t MOST = std::numeric_limits<int>::max() / 2;
+// Blocks of 256 threads, or columns of 64: a launch has less than 2^32 of them.
+constexpr int64_t MOST_BLOCKS = (1 << 24) - 1;
 
 hipStream_t stream() { return at::hip::getCurrentHIPStream().stream(); }
 
@@ -107,7 +109,11 @@ bool tracked(const T&... t) {
     if (!torch::GradMode::is_enabled()) return false;
     const std::initializer_list<OptTensor> all{t...};
     bool any = false;
-    for (const auto& v : all) any = any || (v && v->requires_grad());
+    for (const auto& v : all) {
+        any = any || (v && v->requires_grad());
+        TORCH_CHECK_NOT_IMPLEMENTED(!v || !v->_fw_grad(0).defined(),
+                                    "no forward-mode derivatives: use the reference on CPU");
+    }
     if (any) check_capture(all);
     return any;
 }
@@ -145,7 +151,6 @@ int is_bf16(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 ? 1 : 
 std::tuple<Tensor, Tensor> layer_norm_fwd(const Tensor& x, const Tensor& weight,
                                           const OptTensor& bias, const OptTensor& residual,
                                           double eps) {
-    const c10::DeviceGuard guard(x.device());
     const int64_t dim = x.size(-1), rows = x.numel() / dim;
     auto y = torch::empty_like(x);
     Tensor s;
@@ -203,10 +208,11 @@ struct LayerNormBackward : Node {
 variable_list layer_norm(const Tensor& x, const Tensor& weight, const OptTensor& bias, double eps,
                          const OptTensor& residual) {
     check_first(x, "x");
+    const c10::DeviceGuard guard(x.device());
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x must have a last axis to normalise, got ",
                       x.sizes());
     const int64_t dim = x.size(-1);
-    TORCH_CHECK(dim <= MOST && x.numel() / dim <= MOST, "x is too large");
+    TORCH_CHECK(dim <= MOST_BLOCKS && x.numel() / dim <= MOST, "x is too large");
     check(weight, "weight", x, x.scalar_type(), {dim});
     if (bias) check(*bias, "bias", x, x.scalar_type(), {dim});
     if (residual) check(*residual, "residual", x, x.scalar_type(), x.sizes());
@@ -229,7 +235,6 @@ variable_list layer_norm(const Tensor& x, const Tensor& weight, const OptTensor&
 // ---- K10: gated linear recurrence ------------------------------------------
 std::tuple<Tensor, Tensor, Tensor> gated_recurrence_fwd(const Tensor& gates, const OptTensor& h0,
                                                         const OptTensor& lengths, bool keep) {
-    const c10::DeviceGuard guard(gates.device());
     const int64_t T = gates.size(0), B = gates.size(1), H = gates.size(2) / 3;
     const auto f32 = gates.options().dtype(torch::kFloat32);
     auto y = torch::empty({T, B, H}, gates.options());
@@ -289,6 +294,7 @@ struct GatedRecurrenceBackward : Node {
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const OptTensor& h0,
                                             const OptTensor& lengths) {
     check_first(gates, "gates");
+    const c10::DeviceGuard guard(gates.device());
     TORCH_CHECK_VALUE(gates.dim() == 3 && gates.size(2) % 3 == 0,
                       "gates must be [T, B, 3H], got ", gates.sizes());
     const int64_t T = gates.size(0), B = gates.size(1), H = gates.size(2) / 3;
@@ -328,7 +334,6 @@ LinearSizes sizes_of(const Tensor& x, const Tensor& weight) {
 }
 
 Tensor gated_linear_fwd(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
-    const c10::DeviceGuard guard(x.device());
     const auto n = sizes_of(x, weight);
     auto y = torch::empty(n.out, x.options());
     const int rc = launch_gated_linear_fwd(is_bf16(x), x.data_ptr(), weight.data_ptr(), ptr(bias),
@@ -380,6 +385,7 @@ struct GatedLinearBackward : Node {
 
 Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
     check_first(x, "x");
+    const c10::DeviceGuard guard(x.device());
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must have a last axis");
     TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(0) % 2 == 0,
                       "weight must be [2F, K], got ", weight.sizes());
@@ -389,9 +395,10 @@ Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
     // tiles of 64 by 64 at the least lie on one grid axis
-    TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST / 2, "x or weight is too large");
+    TORCH_CHECK(M <= MOST && K <= MOST && F <= MOST_BLOCKS, "x or weight is too large");
     const int64_t m = M / 64 + 1, k = K / 64 + 1, f = 2 * F / 64 + 1;
-    TORCH_CHECK(m * f <= MOST && m * k <= MOST && k * f <= MOST, "x or weight is too large");
+    TORCH_CHECK(m * f <= MOST_BLOCKS && m * k <= MOST_BLOCKS && k * f <= MOST_BLOCKS,
+                "x or weight is too large");
     // a tile's places are counted in 32 bits from its first: 256 rows, or a gate's
     // row and its value's
     TORCH_CHECK((F + 256) * K <= MOST && 512 * F <= MOST, "weight is too large");

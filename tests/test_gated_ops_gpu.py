@@ -108,6 +108,24 @@ def test_norm_partial_gradients():
               [norm_oracle(x, w, None, r, g, torch.zeros_like(g))[2]])
 
 
+def test_norm_many_short_rows():
+    run_norm(4_300_000, 3, BF16, False)  # more threads than a launch has, at 1024 a row
+
+
+def test_norm_offsets_past_32_bits():
+    few, times, dim = 1000, 1100, 2048  # 2.25e9 elements
+    x, r = (rand(few, dim, seed=i, dtype=BF16).repeat(times, 1) for i in (0, 1))
+    dy = rand(few, dim, seed=2, dtype=BF16).repeat(times, 1)
+    w, b = rand(dim, seed=3, dtype=BF16), rand(dim, seed=4, dtype=BF16)
+    ins = leaves(x)
+    y, s = layer_norm(x, w, b, residual=r)
+    dx = torch.autograd.grad([y], ins, [dy])[0]
+    want = norm_oracle(x[:few], w, b, r[:few], dy[:few], torch.zeros_like(dy[:few]))
+    for i in (0, times // 2, times - 1):
+        rows = slice(i * few, (i + 1) * few)
+        check_all([y[rows], s[rows], dx[rows]], want[:3])
+
+
 # ------------------------------------------------------------ gated recurrence
 def run_recurrence(T, B, H, dtype, lengths=None, state=True, seed=0):
     gates = rand(T, B, 3 * H, seed=seed, dtype=dtype)
@@ -232,6 +250,21 @@ def test_recurrence_offsets_past_32_bits():
     assert torch.equal(y[:, 0], y[:, -2]) and torch.equal(dg[:, 0], dg[:, -2])
 
 
+def test_recurrence_steps_past_32_bits():
+    """Steps whose gates lie 2^31 values on: the last of them forget the first,
+    as a thousand sigmoids of normal gates multiply to less than 2^-500."""
+    T, tail = 720_000_000, 1000
+    gates = torch.zeros(T, 1, 3, device="cuda", dtype=BF16)
+    gates[-tail:] = rand(tail, 1, 3, dtype=BF16)
+    dy = torch.ones(T, 1, 1, device="cuda", dtype=BF16)
+    ins = leaves(gates)
+    y, hT = gated_recurrence(gates)
+    dg = torch.autograd.grad([y], ins, [dy])[0]
+    want = recurrence_oracle(gates[-tail:], None, None, dy[-tail:], None)
+    check_all([y[-tail:], hT, dg[-tail:]], want[:3])
+    assert not y[:-tail].any()
+
+
 # ----------------------------------------------------------- gated linear unit
 def run_linear(M, K, F, dtype, bias=True, seed=0, shape=None, oracle_on="cpu"):
     x = rand(M, K, seed=seed, dtype=dtype).reshape(shape or (M, K))
@@ -288,6 +321,24 @@ def test_linear_larger(M, K, F, dtype):
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_linear_tiles(M, K, F, dtype):
     run_linear(M, K, F, dtype, seed=K, oracle_on="cuda")
+
+
+def test_linear_offsets_past_32_bits():
+    few, times, K, F = 64, 65600, 520, 16  # 2.2e9 elements
+    x, dy = rand(few, K, dtype=BF16).repeat(times, 1), rand(few, F, seed=1, dtype=BF16).repeat(times, 1)
+    w, b = rand(2 * F, K, seed=2, dtype=BF16, scale=K ** -0.5), rand(2 * F, seed=3, dtype=BF16)
+    ins = leaves(x, w, b)
+    y = gated_linear(x, w, b)
+    dx, dw, db = torch.autograd.grad([y], ins, [dy])
+    want = linear_oracle(x[:few], w, b, dy[:few])
+    for i in (0, times // 2, times - 1):
+        rows = slice(i * few, (i + 1) * few)
+        check_all([y[rows], dx[rows]], want[:2])
+    # Sums over `times` equal blocks of rows: dp is rounded alike in each, as in
+    # run_linear, and the additions' roundings have independent signs.
+    for got, (exact, _) in zip((dw, db), want[2:]):
+        off = (got.double().cpu() / times - exact).norm() / exact.norm()
+        assert off < 2 * torch.finfo(BF16).eps / 2 + (few * times) ** 0.5 * 2.0 ** -24, float(off)
 
 
 def test_linear_shapes_strides_and_partial_gradients():
@@ -366,6 +417,77 @@ def test_second_derivatives_are_refused():
             g.sum().backward()
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum(), x)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x, w = rand(3, 8), rand(8, seed=1)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for op in (lambda: layer_norm(d, w), lambda: gated_linear(d, rand(6, 8, seed=2)),
+                   lambda: gated_recurrence(d.view(1, 1, 24))):
+            with pytest.raises(NotImplementedError):
+                op()
+
+
+def test_a_graph_is_walked_once_unless_retained():
+    p = block_inputs(FP32)
+    x, w, g = p["x"], p["wl"], p["wg"]
+    for op in (lambda: layer_norm(x, p["w1"]), lambda: gated_linear(x, w),
+               lambda: gated_recurrence(x @ g.t())[0]):
+        y = op()
+        first = torch.autograd.grad(y, x, p["dy"], retain_graph=True)[0]
+        again = torch.autograd.grad(y, x, p["dy"])[0]
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, x, p["dy"])
+
+
+def test_saved_tensors_may_live_elsewhere_or_be_computed_again():
+    from torch.utils.checkpoint import checkpoint
+    p = block_inputs(BF16)
+    want = block(p, lambda n: n @ p["wg"].t())
+    with torch.autograd.graph.save_on_cpu():
+        got = block(p, lambda n: n @ p["wg"].t())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+    def run(x):
+        y, hT = gated_recurrence(layer_norm(x, p["w1"], p["b1"]) @ p["wg"].t(), p["h0"])
+        return gated_linear(y, p["wl"], p["bl"])
+
+    a = torch.autograd.grad(run(p["x"]), [p["x"], p["wl"]], p["dy"])
+    b = torch.autograd.grad(checkpoint(run, p["x"], use_reentrant=False), [p["x"], p["wl"]], p["dy"])
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
+
+
+def test_saved_inputs_changed_in_place_are_noticed():
+    x, w, g = rand(3, 8), rand(8, seed=1), rand(2, 3, 12, seed=2)
+    lengths = torch.tensor([2, 1, 0], dtype=torch.int32, device="cuda")
+    for op, change in ((lambda: layer_norm(x, w.requires_grad_(True)), x),
+                       (lambda: gated_linear(x, rand(6, 8, seed=2).requires_grad_(True)), x),
+                       (lambda: gated_recurrence(g.requires_grad_(True), None, lengths)[0], lengths)):
+        y = op()
+        change.add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_one_tensor_in_two_places():
+    x, w = rand(5, 40), rand(40, seed=1)
+    ins = leaves(x, w)
+    y, s = layer_norm(x, w, w, residual=x)
+    assert torch.equal(s, 2 * x)
+    dy, ds = rand(5, 40, seed=2), rand(5, 40, seed=3)
+    dx, dw = torch.autograd.grad([y, s], ins, [dy, ds])
+    want = norm_oracle(x, w, w, x, dy, ds)
+    check_all([y, s], want[:2])
+    check_all([dx, dw], [(2 * want[2][0], 2 * want[2][1]),
+                         (want[3][0] + want[4][0], want[3][1] + want[4][1])])
+    w1 = rand(40, seed=4)  # one axis alone
+    assert torch.equal(layer_norm(x[0], w1), layer_norm(x[:1], w1)[0])
+    w2 = rand(6, 40, seed=5)
+    assert torch.equal(gated_linear(x[0], w2), gated_linear(x[:1], w2)[0])
 
 
 def block(p, gates_of):
