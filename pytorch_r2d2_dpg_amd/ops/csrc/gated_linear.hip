@@ -95,7 +95,7 @@ struct Operand {
     int inside;           // indexes of the tile that exist, K: 1 at least
     int half, other;      // K: indexes from `half` on lie `other` rows further
     unsigned at[ROUNDS];  // this thread's pieces: elements from base on, at k = 0
-    u4 held[DIRECT ? 1 : ROUNDS];
+    u4 held[DIRECT ? 1 : 3][ROUNDS];  // stages on their way through registers
 
     static DEV_INLINE int swizzle(int row, int piece) {
         const int run = row / (4 * JUMP);
@@ -126,7 +126,8 @@ struct Operand {
                 at[r] = (unsigned)((i + (row >= half ? (int64_t)other : 0)) * pitch) + piece_of(r) * P;
             } else {
                 const int i = piece_of(r) * P;
-                at[r] = (unsigned)(row * pitch) + (DIRECT && i >= inside ? inside - P : i);
+                const int last = (inside - 1) / P * P;  // piece
+                at[r] = (unsigned)(row * pitch) + (i < last ? i : last);
             }
         }
     }
@@ -137,9 +138,12 @@ struct Operand {
         else return k0 + row_of(r) >= k_hi ? 0 : DIRECT ? P : inside - piece_of(r) * P;
     }
 
-    // Every piece of the stage exists: unaligned ones may end with the indexes.
+    // Every piece of the stage can be read whole. Unaligned ones may pass a row's
+    // end, into the next row: their values past it belong to results that are not
+    // stored.
     DEV_INLINE bool whole(int k0, int k_hi) const {
-        return k0 + DEPTH<E> <= k_hi && (LIE == Lie::K || DIRECT || SPAN <= inside);
+        if (LIE == Lie::K || DIRECT || SPAN <= inside) return k0 + DEPTH<E> <= k_hi;
+        return k0 + DEPTH<E> < k_hi && pitch >= P;
     }
 
     // One round of a whole stage.
@@ -149,28 +153,30 @@ struct Operand {
                     to + r * THREADS * 16);
     }
 
-    DEV_INLINE void fetch(unsigned stage, int k0, int k_hi) {
+    // A stage straight to LDS. Aligned pitches: a piece exists whole or not at all.
+    DEV_INLINE void fetch(unsigned stage, int k0, int k_hi) const {
         const E* p = base + (LIE == Lie::K ? k0 : k0 * pitch);
-        const bool whole = this->whole(k0, k_hi);
         const unsigned to = stage + __builtin_amdgcn_readfirstlane(threadIdx.x) * 16;
 #pragma unroll
-        for (int r = 0; r < ROUNDS; ++r) {
-            const int n = whole ? P : left(r, k0, k_hi);
-            if constexpr (DIRECT) {
-                // aligned pitches: a piece exists whole or not at all
-                load_to_lds(n > 0 ? (const void*)(p + at[r]) : &nothing, to + r * THREADS * 16);
-            } else {
-                E v[P];
-                load_run<E, P>(p + at[r], n, v);
-                held[r] = __builtin_bit_cast(u4, v);
-            }
-        }
+        for (int r = 0; r < ROUNDS; ++r)
+            load_to_lds(left(r, k0, k_hi) > 0 ? (const void*)(p + at[r]) : &nothing,
+                        to + r * THREADS * 16);
     }
 
-    DEV_INLINE void settle(u4* stage) const {
-        if constexpr (!DIRECT)
+    // A stage by way of registers, element by element where it is not WHOLE.
+    template <bool WHOLE>
+    DEV_INLINE void hold(int set, int k0, int k_hi) {
+        const E* p = base + (LIE == Lie::K ? k0 : k0 * pitch);
 #pragma unroll
-            for (int r = 0; r < ROUNDS; ++r) stage[r * THREADS + threadIdx.x] = held[r];
+        for (int r = 0; r < ROUNDS; ++r) {
+            E v[P];
+            load_run<E, P>(p + at[r], WHOLE ? P : left(r, k0, k_hi), v);
+            held[set][r] = __builtin_bit_cast(u4, v);
+        }
+    }
+    DEV_INLINE void settle(int set, u4* stage) const {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) stage[r * THREADS + threadIdx.x] = held[set][r];
     }
 
     // The piece of the matrix instructions for the 16 indexes of the fragment that
@@ -402,9 +408,15 @@ product_kernel(Args<E> p) {
         a.fetch(to, k0, k_hi);
         b.fetch(to + A::ROOM * 16, k0, k_hi);
     };
-    const auto settle = [&](int place) {
-        a.settle(lds[place]);
-        b.settle(lds[place] + A::ROOM);
+    const auto hold = [&](int set, int k0, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        if (!WHOLE && k0 >= k_hi) return;
+        a.template hold<WHOLE>(set, k0, k_hi);
+        b.template hold<WHOLE>(set, k0, k_hi);
+    };
+    const auto settle = [&](int set, int place) {
+        a.settle(set, lds[place]);
+        b.settle(set, lds[place] + A::ROOM);
     };
     // Fragments in registers: those of b of two stages, of a the next AHEAD + 1.
     constexpr int RING = T::MI < 4 ? T::MI : 2 * T::MI % 4 == 0 ? 4 : 5, AHEAD = RING - 1;
@@ -431,25 +443,18 @@ product_kernel(Args<E> p) {
     // landed when the waves meet at its beginning, and the place of the stage
     // before it is free for the one STAGES - 1 on.
     constexpr int LOADS = DIRECT ? A::ROUNDS + B::ROUNDS : 0;
-    if (k_lo < k_hi) {
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s)
-            if (k_lo + s * BD < k_hi) {
-                fetch(s, k_lo + s * BD);
-                if (!DIRECT && s + 1 < STAGES - 1) settle(s);
-            }
-        if (DIRECT && k_lo + (STAGES - 2) * BD >= k_hi) wait_and_meet<0>();
-        else if (DIRECT) wait_and_meet<(STAGES - 2) * LOADS>();
-        else wait_and_meet<63>();
+    const auto read_first = [&] {
 #pragma unroll
         for (int j = 0; j < T::NI; ++j) read_b(0, j, 0);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) read_a(i, i, 0);
-    }
+    };
     int place = 0;  // of the stage whose products run
     // Two stages from k0 on. SPREAD: all that they wait for and fetch exists whole,
     // and is fetched a round at a time between the products: all at once the loads
-    // hold up the waves until the memory has taken them.
+    // hold up the waves until the memory has taken them. By way of registers a
+    // stage is fetched three ahead and settles in LDS one ahead; without a branch
+    // on the way, behind which the compiler would wait for all loads.
     const auto two_stages = [&](int k0, auto spread) {
         constexpr bool SPREAD = decltype(spread)::value;
 #pragma unroll
@@ -460,8 +465,9 @@ product_kernel(Args<E> p) {
             const int before = place > 0 ? place - 1 : STAGES - 1;
             const unsigned to = lds_at + before * (A::ROOM + B::ROOM) * 16;
             if constexpr (!DIRECT) {
-                if (far - BD < k_hi) settle(before > 0 ? before - 1 : STAGES - 1);
+                if (SPREAD || at + BD < k_hi) settle(s, after);
                 wait_and_meet<63>();
+                hold(s, at + 3 * BD, spread);
             } else if (SPREAD || far - BD < k_hi) {
                 wait_and_meet<(STAGES - 3) * LOADS>();
             } else if (STAGES > 4 && far - 2 * BD < k_hi) {
@@ -469,13 +475,14 @@ product_kernel(Args<E> p) {
             } else {
                 wait_and_meet<0>();
             }
-            if (!SPREAD && far < k_hi) fetch(before, far);
+            if constexpr (DIRECT && !SPREAD)
+                if (far < k_hi) fetch(before, far);
 #pragma unroll
             for (int i = 0; i < T::MI; ++i) {
                 const int now = s * T::MI + i, next = i + AHEAD;
                 read_a((now + AHEAD) % RING, next % T::MI, next < T::MI ? place : after);
                 if (i < T::NI) read_b((s + 1) & 1, i, after);
-                if constexpr (SPREAD)
+                if constexpr (SPREAD && DIRECT)
 #pragma unroll
                     for (int n = i * LOADS / T::MI; n < (i + 1) * LOADS / T::MI; ++n) {
                         if (n < A::ROUNDS) a.fetch_round(n, to, far);
@@ -493,12 +500,41 @@ product_kernel(Args<E> p) {
             place = after;
         }
     };
+    // The first stages, then pairs of them as long as the second one fetches a
+    // whole stage, then the last ones.
+    constexpr int FAR = DIRECT ? STAGES - 1 : 3;
+    const int last = a.whole(k_lo, k_hi) && b.whole(k_lo, k_hi) ? k_hi - (FAR + 2) * BD - !DIRECT
+                                                                : k_lo - 1;
     int k0 = k_lo;
-    if constexpr (DIRECT) {
-        // as long as the second of the two fetches a whole stage
-        const int last = a.whole(k_lo, k_hi) && b.whole(k_lo, k_hi) ? k_hi - (STAGES + 1) * BD : k_lo - 1;
+    const auto main_loop = [&] {
 #pragma unroll 1
         for (; k0 <= last; k0 += 2 * BD) two_stages(k0, std::true_type());
+    };
+    if constexpr (DIRECT) {
+        if (k_lo < k_hi) {
+#pragma unroll
+            for (int s = 0; s < STAGES - 1; ++s)
+                if (k_lo + s * BD < k_hi) fetch(s, k_lo + s * BD);
+            if (k_lo + (STAGES - 2) * BD >= k_hi) wait_and_meet<0>();
+            else wait_and_meet<(STAGES - 2) * LOADS>();
+            read_first();
+            main_loop();
+        }
+    } else {
+        const auto begin = [&](auto whole) {
+            hold(2, k_lo, whole);
+            hold(0, k_lo + BD, whole);
+            hold(1, k_lo + 2 * BD, whole);
+            settle(2, 0);
+            wait_and_meet<63>();
+            read_first();
+        };
+        if (k_lo <= last) {
+            begin(std::true_type());
+            main_loop();
+        } else if (k_lo < k_hi) {
+            begin(std::false_type());
+        }
     }
 #pragma unroll 1
     for (; k0 < k_hi; k0 += 2 * BD) two_stages(k0, std::false_type());
