@@ -11,8 +11,13 @@
 // each other's maps through LDS and then walk their own steps with the state
 // that they start from: every input is read once and time runs in parallel.
 // Bound by memory: 80 steps of 256 rows of 512 in bf16 take 20 us forward and
-// 36 us backward on the MI355X, 4.4 and 4.3 TB/s. Where the channels are too few to fill the card, time is split over blocks
-// as well: one launch reduces each segment to its map, and the next walks.
+// 30 us backward on the MI355X, 4.5 and 5.1 TB/s, where a copy of 2 GiB reaches
+// 4.9. Where the channels are too few to fill the card, time is split over blocks
+// as well: one launch reduces each segment to its map, and the next walks. The
+// gates are read twice then: 16384 steps of 4 rows take 41 + 57 and 49 + 94 us.
+// Blocks that wait for each other's states could read them once, but would join
+// them in the order in which they arrive, and the result would change from run
+// to run.
 //
 // The forward pass keeps the state that each chunk starts from, in 32 bits,
 // 1/CHUNK of the steps: the backward pass walks the chunk again from it in
@@ -410,8 +415,9 @@ recurrence_bwd_kernel(Args<E> p) {
 
 // How time is laid over waves and blocks; a tile is 64 lanes' channels. Four
 // waves a SIMD hide the memory's latency, so a block has the 4 to 8 waves that
-// bring the launch to WAVES. Measured in bf16, H = 512, forward and backward:
-// 1024 tiles of 80 steps 20 and 36 us with 4 waves, 21 and 46 with 5; 256 tiles
+// bring the launch to WAVES. Measured in bf16, H = 512, forward and backward, side
+// by side when the rule was made: 1024 tiles of 80 steps 20 and 36 us with 4
+// waves, 21 and 46 with 5; 256 tiles
 // of 200 steps 16 and 26 with 7, 20 and 32 with 4. Where 8 waves leave the card
 // half empty and take three passes or more, the chunks are dealt out to
 // `segments` blocks of 4 waves: 64 tiles of 256 steps take 11 and 17 us in 8
