@@ -118,15 +118,14 @@ DEV_INLINE float wave_sum(float v) {
 
 // out[c] = sum over r of part[r][c] in a fixed order: the second stage of a
 // reduction over rows, in place of atomics whose order would change results.
-// A block has 16 columns, which 64 groups of threads walk 64 rows apart, eight
-// loads at a time.
+// A block of 1024 threads has 16 columns, which 64 groups of threads walk 64 rows
+// apart, eight loads at a time.
 template <typename E>
-static __global__ void __launch_bounds__(1024)
-column_sum_kernel(const float* __restrict__ part, E* __restrict__ out,
-                  int rows, int cols) {
+DEV_INLINE void sum_columns(const float* __restrict__ part, E* __restrict__ out, int rows,
+                            int cols, int block) {
     __shared__ float sums[64][17];
     const int in = threadIdx.x & 15, group = threadIdx.x >> 4;
-    const int c = blockIdx.x * 16 + in;
+    const int c = block * 16 + in;
     const float* p = part + (c < cols ? c : cols - 1);
     float s = 0.0f;
     for (int r0 = group; r0 < rows; r0 += 8 * 64) {
@@ -148,10 +147,4 @@ column_sum_kernel(const float* __restrict__ part, E* __restrict__ out,
         out[c] = from_f<E>((t[0] + t[1]) + (t[2] + t[3]));
     }
 }
-
-template <typename E>
-static int column_sum(const float* part, E* out, int rows, int cols, hipStream_t st) {
-    if (cols) column_sum_kernel<E><<<(cols + 15) / 16, 1024, 0, st>>>(part, out, rows, cols);
-    LSTM_CHECK_LAUNCH();
-    return 0;
-}
+constexpr int column_blocks(int cols) { return cols / 16 + (cols % 16 != 0); }

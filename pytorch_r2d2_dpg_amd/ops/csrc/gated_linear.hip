@@ -561,28 +561,49 @@ product_kernel(Args<E> p) {
         finish<E, T, END, false>(p, acc, tm, m0, n0, lds);
 }
 
-// out = sum over the splits of part, in their order.
+// out[i] = sum over the splits of part [splits, n], in their order.
 template <typename E>
-__global__ void __launch_bounds__(256)
-join_splits_kernel(const float* __restrict__ part, E* __restrict__ out, int64_t n, int splits) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
-    const int have = n - i < 4 ? (int)(n - i) : 4;
+struct Splits {
+    const float* part;
+    E* out;
+    int64_t n;
+    int splits;  // 1: the product has written the result itself
+    int blocks() const { return splits > 1 ? (int)((n + 4095) / 4096) : 0; }
+};
+
+template <typename E>
+DEV_INLINE void join_splits(const Splits<E>& q, int block) {
+    const int64_t i = ((int64_t)block * 1024 + threadIdx.x) * 4;
+    if (i >= q.n) return;
+    const int have = q.n - i < 4 ? (int)(q.n - i) : 4;
     float s[4] = {}, v[8][4];
-    for (int z0 = 0; z0 < splits; z0 += 8) {
+    for (int z0 = 0; z0 < q.splits; z0 += 8) {
 #pragma unroll
         for (int z = 0; z < 8; ++z)
-            if (z0 + z < splits) load_run<float, 4>(part + (z0 + z) * n + i, have, v[z]);
+            if (z0 + z < q.splits) load_run<float, 4>(q.part + (z0 + z) * q.n + i, have, v[z]);
 #pragma unroll
         for (int z = 0; z < 8; ++z)
-            if (z0 + z < splits)
+            if (z0 + z < q.splits)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) s[q] += v[z][q];
+                for (int k = 0; k < 4; ++k) s[k] += v[z][k];
     }
     E o[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = from_f<E>(s[q]);
-    store_run<E, 4>(out + i, have, o);
+    for (int k = 0; k < 4; ++k) o[k] = from_f<E>(s[k]);
+    store_run<E, 4>(q.out + i, have, o);
+}
+
+// What the products of the backward pass leave in parts, in one launch: three
+// would take a small batch longer than their work.
+template <typename E>
+__global__ void __launch_bounds__(1024)
+join_kernel(Splits<E> dx, int dx_blocks, Splits<E> dw, int dw_blocks,
+            const float* __restrict__ part_db, E* __restrict__ db, int rows, int cols) {
+    int block = blockIdx.x;
+    if (block < dx_blocks) return join_splits(dx, block);
+    block -= dx_blocks;
+    if (block < dw_blocks) return join_splits(dw, block);
+    sum_columns<E>(part_db, db, rows, cols, block - dw_blocks);
 }
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -611,7 +632,7 @@ void each_tile(F&& f) {
 }
 
 // How a product is cut: which tile, and into how many splits of k, whose sums
-// join_splits_kernel adds.
+// join_kernel adds.
 struct Cut {
     int bm, bn, splits;
 };
@@ -676,17 +697,13 @@ int product(const Args<E>& p, Cut cut, hipStream_t st) {
     return rc;
 }
 
-// A plain product, in one piece or in splits through `part`.
+// A plain product to `out`, in one piece or in splits, for the join, through its part.
 template <typename E, Lie LA, Lie LB>
-int plain(Args<E> p, Cut cut, float* part, hipStream_t st) {
-    if (cut.splits == 1) return product<E, LA, LB, End::PLAIN>(p, cut, st);
-    p.part = part;
-    const int rc = product<E, LA, LB, End::PART>(p, cut, st);
-    if (rc) return rc;
-    const int64_t n = (int64_t)p.M * p.N;
-    join_splits_kernel<E><<<ceil_div(n, 1024), 256, 0, st>>>(part, p.out, n, cut.splits);
-    LSTM_CHECK_LAUNCH();
-    return 0;
+int plain(Args<E> p, Cut cut, const Splits<E>& to, hipStream_t st) {
+    p.out = to.out;
+    p.part = const_cast<float*>(to.part);
+    return to.splits == 1 ? product<E, LA, LB, End::PLAIN>(p, cut, st)
+                          : product<E, LA, LB, End::PART>(p, cut, st);
 }
 
 template <typename E> Cut cut_gated(int M, int K, int F) {
@@ -717,13 +734,19 @@ int bias_parts(int M, int K, int F) {
     return ceil_div(M, cut_gated<E>(M, K, F).bm);
 }
 
-// Floats of partial sums for the splits of dx and dw, which take turns with them.
+// The splits of dx and dw, whose partial sums lie one behind the other.
+template <typename E>
+void splits_of(int M, int K, int F, E* dx, E* dw, const float* part, Splits<E>& x, Splits<E>& w) {
+    x = {part, dx, (int64_t)M * K, dx ? cut_dx<E>(M, K, F).splits : 1};
+    const int64_t before = x.splits > 1 ? x.splits * x.n : 0;
+    w = {part + before, dw, 2 * (int64_t)F * K, dw ? cut_dw<E>(M, K, F).splits : 1};
+}
+
+// Floats of those partial sums.
 template <typename E>
 int64_t split_sums(int M, int K, int F, bool dx, bool dw) {
-    const int sx = cut_dx<E>(M, K, F).splits, sw = cut_dw<E>(M, K, F).splits;
-    const int64_t nx = dx && sx > 1 ? (int64_t)sx * M * K : 0;
-    const int64_t nw = dw && sw > 1 ? (int64_t)sw * 2 * F * K : 0;
-    return nx > nw ? nx : nw;
+    const int64_t x = dx ? cut_dx<E>(M, K, F).splits : 1, w = dw ? cut_dw<E>(M, K, F).splits : 1;
+    return (x > 1 ? x * M * K : 0) + (w > 1 ? w * 2 * F * K : 0);
 }
 
 template <typename E>
@@ -739,28 +762,29 @@ int bwd(const void* x, const void* w, const void* bias, const void* dy, void* dp
         rc = product<E, Lie::K, Lie::K, End::GATED_GRAD>(p, cut_gated<E>(M, K, F), st);
         if (rc) return rc;
     }
-    if (db && F) {
-        rc = column_sum<E>(part_db, (E*)db, bias_parts<E>(M, K, F), 2 * F, st);
-        if (rc) return rc;
-    }
-    if (dx && (int64_t)M * K != 0) {
+    Splits<E> sx, sw;
+    splits_of<E>(M, K, F, (E*)dx, (E*)dw, part, sx, sw);
+    if (dx && sx.n) {
         Args<E> p{};
         p.a = (const E*)dp; p.pitch_a = 2 * (int64_t)F;
         p.b = (const E*)w; p.pitch_b = K;
         p.M = M; p.N = K; p.K = 2 * F;
-        p.out = (E*)dx;
-        rc = plain<E, Lie::K, Lie::INDEX>(p, cut_dx<E>(M, K, F), part, st);
+        rc = plain<E, Lie::K, Lie::INDEX>(p, cut_dx<E>(M, K, F), sx, st);
         if (rc) return rc;
     }
-    if (dw && (int64_t)F * K != 0) {
+    if (dw && sw.n) {
         Args<E> p{};
         p.a = (const E*)dp; p.pitch_a = 2 * (int64_t)F;
         p.b = (const E*)x; p.pitch_b = K;
         p.M = 2 * F; p.N = K; p.K = M;
-        p.out = (E*)dw;
-        rc = plain<E, Lie::INDEX, Lie::INDEX>(p, cut_dw<E>(M, K, F), part, st);
+        rc = plain<E, Lie::INDEX, Lie::INDEX>(p, cut_dw<E>(M, K, F), sw, st);
         if (rc) return rc;
     }
+    const int bx = sx.blocks(), bw = sw.blocks(), bb = db ? column_blocks(2 * F) : 0;
+    if (bx + bw + bb == 0) return 0;
+    join_kernel<E><<<bx + bw + bb, 1024, 0, st>>>(sx, bx, sw, bw, part_db, (E*)db,
+                                                  bias_parts<E>(M, K, F), 2 * F);
+    LSTM_CHECK_LAUNCH();
     return 0;
 }
 

@@ -345,6 +345,12 @@ norm_dw_long_kernel(const E* __restrict__ x, const E* __restrict__ res,
     part[((int64_t)blockIdx.y * 2 + 1) * dim + c] = db;
 }
 
+template <typename E>
+__global__ void __launch_bounds__(1024)
+column_sum_kernel(const float* __restrict__ part, E* __restrict__ out, int rows, int cols) {
+    sum_columns<E>(part, out, rows, cols, blockIdx.x);
+}
+
 // By the runs of a row, the smallest group of threads that holds it with two
 // runs a thread: in bf16 more leave the registers of one wave a SIMD. 0 threads:
 // longer than 8192 elements, or shorter than a run.
@@ -444,7 +450,9 @@ int bwd(const void* x, const void* res, const void* w, const void* dy, const voi
         });
     }
     LSTM_CHECK_LAUNCH();
-    return column_sum<E>(part, (E*)dwb, parts, 2 * dim, st);
+    column_sum_kernel<E><<<column_blocks(2 * dim), 1024, 0, st>>>(part, (E*)dwb, parts, 2 * dim);
+    LSTM_CHECK_LAUNCH();
+    return 0;
 }
 
 }  // namespace
