@@ -1,4 +1,4 @@
-// Python bindings for the MI355X HIP kernels (K1-K7).
+// Python bindings for the MI355X HIP kernels (K1-K7; K9-K11 in bindings_gated.cpp).
 // Pure C++ TU: talks to the .hip translation units through extern "C"
 // launchers taking raw pointers + the current HIP stream from torch.
 
