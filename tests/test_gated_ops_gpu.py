@@ -306,6 +306,14 @@ def test_linear_widths(K, F, dtype):
     run_linear(70, K, F, dtype, bias=F != 16, seed=K + F)
 
 
+# rows shorter than a load, in loops long enough to leave their ends
+@pytest.mark.parametrize("K", [1, 3, 4, 5, 9])
+@pytest.mark.parametrize("F", [1, 2, 3, 5])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_linear_narrow(K, F, dtype):
+    run_linear(700, K, F, dtype, seed=K + F)
+
+
 @pytest.mark.parametrize("M, K, F", [(1500, 512, 1024), (5000, 96, 64), (33, 2048, 512), (8200, 136, 1032), (8195, 67, 1029)])
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_linear_larger(M, K, F, dtype):
