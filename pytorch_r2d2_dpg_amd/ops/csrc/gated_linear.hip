@@ -249,10 +249,11 @@ DEV_INLINE void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
     tn = in / rows;
 }
 
-// BM x BN of a result by WM x WN waves, with STAGES of the operands in LDS. Four
-// stages of 64 bytes a row hide a load behind two to three others; the largest
-// tile has the LDS for a fifth (16384 x 2048 x 4096: 436 us, 457 with two stages
-// of 128 bytes), which gains nothing in the smaller ones.
+// BM x BN of a result by WM x WN waves, with STAGES of the operands in LDS, of 64
+// bytes a row. A fifth one fits with the largest tile (16384 x 2048 x 4096: 436 us,
+// 457 with two stages of 128 bytes) and with four blocks of the smallest, whose few
+// rows wait for the weights from memory (16 x 2048 x 4096: 11.5 us, 15.2 with four);
+// between them it gained nothing.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_ = 4>
 struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
@@ -561,36 +562,58 @@ product_kernel(Args<E> p) {
         finish<E, T, END, false>(p, acc, tm, m0, n0, lds);
 }
 
-// out[i] = sum over the splits of part [splits, n], in their order.
+// out[i] = sum over the splits of part [splits, n], in a fixed order.
 template <typename E>
 struct Splits {
     const float* part;
     E* out;
     int64_t n;
     int splits;  // 1: the product has written the result itself
-    int blocks() const { return splits > 1 ? (int)((n + 4095) / 4096) : 0; }
+    // Groups of a block's threads, which add every GROUPS-th split of the same
+    // results. Four where the results are few and their splits many: 128 x 64 of 64
+    // splits take 10 us with the product, 18 with one group, but 2048 x 512 of 8
+    // take 58 in place of 55.
+    __host__ __device__ bool grouped() const { return splits >= 8 && n <= 1 << 19; }
+    int blocks() const {
+        const int each = grouped() ? 1024 : 4096;
+        return splits > 1 ? (int)((n + each - 1) / each) : 0;
+    }
 };
 
-template <typename E>
+template <typename E, int GROUPS>
 DEV_INLINE void join_splits(const Splits<E>& q, int block) {
-    const int64_t i = ((int64_t)block * 1024 + threadIdx.x) * 4;
-    if (i >= q.n) return;
-    const int have = q.n - i < 4 ? (int)(q.n - i) : 4;
-    float s[4] = {}, v[8][4];
-    for (int z0 = 0; z0 < q.splits; z0 += 8) {
+    constexpr int THREADS = 1024 / GROUPS;
+    const int group = threadIdx.x / THREADS, in = threadIdx.x % THREADS;
+    const int64_t i = ((int64_t)block * THREADS + in) * 4, left = q.n - i;
+    const int have = left < 0 ? 0 : left < 4 ? (int)left : 4;
+    f4 s = {};
+    float v[8][4];
+    for (int z0 = group; z0 < q.splits; z0 += 8 * GROUPS) {
 #pragma unroll
         for (int z = 0; z < 8; ++z)
-            if (z0 + z < q.splits) load_run<float, 4>(q.part + (z0 + z) * q.n + i, have, v[z]);
+            if (z0 + GROUPS * z < q.splits)
+                load_run<float, 4>(q.part + (z0 + GROUPS * z) * q.n + i, have, v[z]);
 #pragma unroll
         for (int z = 0; z < 8; ++z)
-            if (z0 + z < q.splits)
+            if (z0 + GROUPS * z < q.splits) s += f4{v[z][0], v[z][1], v[z][2], v[z][3]};
+    }
+    if constexpr (GROUPS > 1) {
+        __shared__ f4 sums[GROUPS][THREADS];
+        sums[group][in] = s;
+        __syncthreads();
+        if (group) return;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s[k] += v[z][k];
+        for (int g = 1; g < GROUPS; ++g) s += sums[g][in];
     }
     E o[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[k] = from_f<E>(s[k]);
     store_run<E, 4>(q.out + i, have, o);
+}
+template <typename E>
+DEV_INLINE void join_splits(const Splits<E>& q, int block) {
+    if (q.grouped()) join_splits<E, 4>(q, block);
+    else join_splits<E, 1>(q, block);
 }
 
 // What the products of the backward pass leave in parts, in one launch: three
@@ -624,7 +647,7 @@ void each_tile(F&& f) {
         f(Tile<160, 256, 2, 4>(), Rate{1, 4.5, 0});
         f(Tile<128, 256, 2, 4>(), Rate{1, 4.3, 0});
         f(Tile<128, 128, 2, 2>(), Rate{2, 3.5, 0.4});
-        f(Tile<64, 64, 2, 2>(), Rate{4, 2.0, 0.25});
+        f(Tile<64, 64, 2, 2, 5>(), Rate{4, 2.0, 0.25});
     } else {
         f(Tile<128, 128, 2, 2>(), Rate{2, 0.5, 1.1});
         f(Tile<64, 64, 2, 2>(), Rate{4, 0.47, 0.38});
