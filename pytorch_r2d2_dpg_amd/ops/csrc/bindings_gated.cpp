@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 
 #include <hip/hip_runtime.h>
@@ -103,17 +104,23 @@ void check_capture(std::initializer_list<OptTensor> inputs) {
     }
 }
 
+// A call that carries tangents, which the kernels would drop. Forward mode has a
+// switch of its own: inference mode turns it off, no_grad does not.
+template <typename... T>
+void check_modes(const T&... t) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const auto& v : std::initializer_list<OptTensor>{t...})
+        TORCH_CHECK_NOT_IMPLEMENTED(!v || !v->_fw_grad(0).defined(),
+                                    "no forward-mode derivatives: use the reference on CPU");
+}
+
 // Whether a gradient may be asked for: then the leaves are looked at too.
 template <typename... T>
 bool tracked(const T&... t) {
     if (!torch::GradMode::is_enabled()) return false;
     const std::initializer_list<OptTensor> all{t...};
     bool any = false;
-    for (const auto& v : all) {
-        any = any || (v && v->requires_grad());
-        TORCH_CHECK_NOT_IMPLEMENTED(!v || !v->_fw_grad(0).defined(),
-                                    "no forward-mode derivatives: use the reference on CPU");
-    }
+    for (const auto& v : all) any = any || (v && v->requires_grad());
     if (any) check_capture(all);
     return any;
 }
@@ -207,6 +214,7 @@ struct LayerNormBackward : Node {
 
 variable_list layer_norm(const Tensor& x, const Tensor& weight, const OptTensor& bias, double eps,
                          const OptTensor& residual) {
+    check_modes(x, weight, bias, residual);
     check_first(x, "x");
     const c10::DeviceGuard guard(x.device());
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x must have a last axis to normalise, got ",
@@ -293,6 +301,7 @@ struct GatedRecurrenceBackward : Node {
 
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const OptTensor& h0,
                                             const OptTensor& lengths) {
+    check_modes(gates, h0);
     check_first(gates, "gates");
     const c10::DeviceGuard guard(gates.device());
     TORCH_CHECK_VALUE(gates.dim() == 3 && gates.size(2) % 3 == 0,
@@ -384,6 +393,7 @@ struct GatedLinearBackward : Node {
 };
 
 Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+    check_modes(x, weight, bias);
     check_first(x, "x");
     const c10::DeviceGuard guard(x.device());
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must have a last axis");
