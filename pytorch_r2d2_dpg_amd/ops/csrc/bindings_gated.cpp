@@ -15,9 +15,12 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <hip/hip_runtime.h>
 
@@ -104,10 +107,28 @@ void check_capture(std::initializer_list<OptTensor> inputs) {
     }
 }
 
-// A call that carries tangents, which the kernels would drop. Forward mode has a
-// switch of its own: inference mode turns it off, no_grad does not.
+// Whether torch's operations are being recorded or only simulated: by jit.trace,
+// make_fx (before or after dispatch), fake or functional tensors. The allocation of
+// an output would be recorded, and not the launch that fills it. Modes that only
+// watch are none of these.
+bool recorded() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Mode = c10::impl::TorchDispatchModeKey;
+    if (torch::jit::tracer::isTracing()) return true;
+    if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) return true;
+    if (!Modes::any_modes_set()) return false;
+    return Modes::get_mode(Mode::PROXY) || Modes::get_mode(Mode::FAKE) ||
+           Modes::get_mode(Mode::FUNCTIONAL);
+}
+
+// What a launch that torch's dispatcher does not see cannot serve: a recording, and
+// tangents, which the kernels would drop. Forward mode has a switch of its own:
+// inference mode turns it off, no_grad does not.
 template <typename... T>
 void check_modes(const T&... t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!recorded(), "the kernels' launches cannot be recorded (traced, "
+                                             "exported or run on fake tensors): use the "
+                                             "reference on CPU");
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const auto& v : std::initializer_list<OptTensor>{t...})
         TORCH_CHECK_NOT_IMPLEMENTED(!v || !v->_fw_grad(0).defined(),

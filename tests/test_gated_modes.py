@@ -54,3 +54,68 @@ def test_tangents_are_refused(grad):
                 op(d)
             with torch.inference_mode():  # torch itself carries no tangent here
                 assert torch.equal(op(d), op(x))
+
+
+# ------------------------------------------------------------------- recording
+def recorders():
+    """Ways of recording a function's torch operations, by name."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def fake(f, x):
+        mode = FakeTensorMode(allow_non_fake_inputs=True)
+        with mode:
+            return f(x)
+
+    def functional(f, x):
+        from torch._subclasses.functional_tensor import FunctionalTensorMode
+        with FunctionalTensorMode():
+            return f(x)
+
+    return {
+        "jit.trace": lambda f, x: torch.jit.trace(f, (x,), check_trace=False),
+        "make_fx": lambda f, x: make_fx(f)(x),
+        "make_fx, before dispatch": lambda f, x: make_fx(f, pre_dispatch=True)(x),
+        "make_fx of fake tensors": lambda f, x: make_fx(f, tracing_mode="fake")(x),
+        "fake tensors": fake,
+        "functional tensors": functional,
+    }
+
+
+RECORDERS = ["jit.trace", "make_fx", "make_fx, before dispatch", "make_fx of fake tensors",
+             "fake tensors", "functional tensors"]
+
+
+@built
+@pytest.mark.parametrize("way", RECORDERS)
+def test_bindings_refuse_to_be_recorded(way):
+    """A recording has the outputs' allocations, and not the launch that fills them.
+    Looked for before the device is, so that this shows without a GPU."""
+    for x, binding, _ in args():
+        with pytest.raises(NotImplementedError, match="recorded"):
+            recorders()[way](binding, x)
+
+
+@pytest.mark.parametrize("way", ["jit.trace", "make_fx"])
+def test_references_can_be_recorded(way):
+    for x, _, op in args():
+        other = x + 1
+        assert torch.equal(recorders()[way](op, x)(other), op(other))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", RECORDERS)
+def test_recording_is_refused(way):
+    for x, _, op in args("cuda"):
+        with pytest.raises(NotImplementedError, match="recorded"):
+            recorders()[way](op, x)
+        assert op(x).isfinite().all()  # and nothing of it stays
+
+
+@pytest.mark.gpu
+def test_modes_that_only_watch_are_served():
+    from torch.utils.flop_counter import FlopCounterMode
+    for x, _, op in args("cuda"):
+        want = op(x)
+        with FlopCounterMode(display=False):
+            assert torch.equal(op(x), want)
