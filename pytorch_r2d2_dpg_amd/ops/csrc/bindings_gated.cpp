@@ -123,7 +123,8 @@ bool recorded() {
 
 // What a launch that torch's dispatcher does not see cannot serve: a recording, and
 // tangents, which the kernels would drop. Forward mode has a switch of its own:
-// inference mode turns it off, no_grad does not.
+// inference mode turns it off, no_grad does not. Both passes look: a recording or a
+// tangent may begin with the outputs' gradients.
 template <typename... T>
 void check_modes(const T&... t) {
     TORCH_CHECK_NOT_IMPLEMENTED(!recorded(), "the kernels' launches cannot be recorded (traced, "
@@ -131,7 +132,7 @@ void check_modes(const T&... t) {
                                              "reference on CPU");
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const auto& v : std::initializer_list<OptTensor>{t...})
-        TORCH_CHECK_NOT_IMPLEMENTED(!v || !v->_fw_grad(0).defined(),
+        TORCH_CHECK_NOT_IMPLEMENTED(!v || !v->defined() || !v->_fw_grad(0).defined(),
                                     "no forward-mode derivatives: use the reference on CPU");
 }
 
@@ -220,6 +221,7 @@ struct LayerNormBackward : Node {
         residual.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
+        check_modes(grads[0], grads.size() > 1 ? grads[1] : Tensor());
         const std::lock_guard<std::mutex> lock(mutex_);
         const Tensor in = x.unpack();
         const OptTensor res = optional(residual);
@@ -308,6 +310,7 @@ struct GatedRecurrenceBackward : Node {
         lengths.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
+        check_modes(grads[0], grads[1]);
         const std::lock_guard<std::mutex> lock(mutex_);
         const Tensor g = gates.unpack();
         const Tensor dy = grads[0].defined()
@@ -404,6 +407,7 @@ struct GatedLinearBackward : Node {
         bias.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
+        check_modes(grads[0]);
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         return once(gated_linear_bwd(x.unpack(), weight.unpack(), optional(bias),

@@ -119,3 +119,40 @@ def test_modes_that_only_watch_are_served():
         want = op(x)
         with FlopCounterMode(display=False):
             assert torch.equal(op(x), want)
+
+
+# ----------------------------------------------------------- the backward pass
+@pytest.mark.gpu
+def test_a_gradient_with_a_tangent_is_refused():
+    """Forward mode through the backward pass alone: the outputs' gradients carry the
+    tangents, of either output of an operator with two."""
+    for i, (x, _, op) in enumerate(args("cuda")):
+        x.requires_grad_(True)
+        y = op(x)
+        dy = torch.ones_like(y)
+        with fwd.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, x, fwd.make_dual(dy, dy), retain_graph=True)
+        assert torch.autograd.grad(y, x, dy)[0].isfinite().all()
+    x, g = torch.randn(3, 8, device="cuda"), torch.randn(2, 3, 6, device="cuda", requires_grad=True)
+    r = torch.randn(3, 8, device="cuda", requires_grad=True)
+    for second, leaf in ((layer_norm(x, torch.ones(8, device="cuda"), residual=r)[1], r),
+                         (gated_recurrence(g)[1], g)):
+        with fwd.dual_level():
+            d = fwd.make_dual(torch.ones_like(second), torch.ones_like(second))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(second, leaf, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before", [False, True])
+def test_recording_the_backward_pass_is_refused(before):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for x, _, op in args("cuda"):
+        x.requires_grad_(True)
+        y = op(x)
+        dy = torch.ones_like(y)
+        back = make_fx(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0], pre_dispatch=before)
+        with pytest.raises(NotImplementedError, match="recorded"):
+            back(dy)
+        assert torch.autograd.grad(y, x, dy)[0].isfinite().all()
