@@ -138,7 +138,13 @@ def gated_recurrence_ref(gates, h0=None, lengths=None):
     y = 0. Returns (y [T,B,H], hT [B,H] in 32 bits at least). Differentiable."""
     wide = torch.promote_types(gates.dtype, torch.float32)
     T, B, H3 = gates.shape
-    f, v, o = gates.to(wide).unflatten(-1, (3, H3 // 3)).unbind(2)
+    gates_w = gates.to(wide)
+    if lengths is not None:
+        # a pad's gates leave before anything is computed of them: the gradient of
+        # what is computed and then not chosen is 0 times what they hold
+        pad = torch.arange(T, device=gates.device)[:, None] >= lengths[None, :]
+        gates_w = gates_w.masked_fill(pad.unsqueeze(2), 0.0)
+    f, v, o = gates_w.unflatten(-1, (3, H3 // 3)).unbind(2)
     h = gates.new_zeros(B, H3 // 3, dtype=wide) if h0 is None else h0.to(wide)
     ys = []
     for t in range(T):
