@@ -29,6 +29,8 @@ def gated_linear(
     """
     if x.is_cuda:
         return hip_ext().gated_linear(x, weight, bias)
+    if not x.is_floating_point():
+        raise TypeError(f"x must be of a floating type, got {x.dtype}")
     if x.dim() == 0:
         raise ValueError("x must have a last axis")
     if weight.dim() != 2 or weight.shape[0] % 2 or weight.shape[1] != x.shape[-1]:

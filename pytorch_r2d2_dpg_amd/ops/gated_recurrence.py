@@ -33,6 +33,8 @@ def gated_recurrence(
     """
     if gates.is_cuda:
         return hip_ext().gated_recurrence(gates, h0, lengths)
+    if not gates.is_floating_point():
+        raise TypeError(f"gates must be of a floating type, got {gates.dtype}")
     if gates.dim() != 3 or gates.shape[2] % 3:
         raise ValueError(f"gates must be [T, B, 3H], got {tuple(gates.shape)}")
     B, H = gates.shape[1], gates.shape[2] // 3

@@ -34,6 +34,8 @@ def layer_norm(
     if x.is_cuda:
         out = hip_ext().layer_norm(x, weight, bias, eps, residual)
         return out[0] if residual is None else (out[0], out[1])
+    if not x.is_floating_point():
+        raise TypeError(f"x must be of a floating type, got {x.dtype}")
     D = x.shape[-1] if x.dim() else 0
     if D == 0:
         raise ValueError(f"x must have a last axis to normalise (got {tuple(x.shape)})")

@@ -34,3 +34,17 @@ def test_recurrence_pads_have_no_effect(fill, dtype):
     for b, n in enumerate(lengths.tolist()):
         assert not y[n:, b].any() and not dgates[n:, b].any()
     assert torch.equal(hT[0], rand(B, H, seed=1)[0]) and torch.equal(dh0[0], rand(B, H, seed=3)[0])
+
+
+def ints(*shape, dtype):
+    return torch.ones(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.uint8, torch.bool, torch.complex64])
+def test_types_that_are_not_real_floats_are_refused(dtype):
+    """Results rounded to whole numbers would be wrong without an error."""
+    for call in (lambda: layer_norm(ints(2, 4, dtype=dtype), ints(4, dtype=dtype)),
+                 lambda: gated_recurrence(ints(2, 2, 6, dtype=dtype)),
+                 lambda: gated_linear(ints(2, 4, dtype=dtype), ints(6, 4, dtype=dtype))):
+        with pytest.raises(TypeError, match="floating"):
+            call()
