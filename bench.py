@@ -32,6 +32,7 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from pytorch_r2d2_dpg_amd.config import Config
 from pytorch_r2d2_dpg_amd.envs import make_env
 from pytorch_r2d2_dpg_amd.learner import Learner
+from pytorch_r2d2_dpg_amd.models import state_dtype
 from pytorch_r2d2_dpg_amd.parallel.dist import DistContext
 from pytorch_r2d2_dpg_amd.replay.gpu_buffer import GpuSequenceReplay
 
@@ -142,13 +143,14 @@ def main() -> int:
     torch.manual_seed(cfg.learner.seed + rank)
     spec = make_env(cfg.env.name).spec
 
+    store_dtype = torch.bfloat16 if args.dtype == "bf16" else torch.float32
     replay = GpuSequenceReplay(
         capacity=cfg.replay.capacity, stored_len=cfg.replay.seq_len + cfg.replay.n_step,
         obs_shape=spec.obs_shape, action_dim=spec.action_dim,
         hidden_size=cfg.model.hidden_size, per_alpha=cfg.replay.per_alpha,
         device=device, seed=cfg.learner.seed + 17 * rank,
         obs_dtype=torch.uint8 if spec.pixel else torch.float32,
-        store_dtype=torch.bfloat16 if args.dtype == "bf16" else torch.float32,
+        store_dtype=store_dtype, state_dtype=state_dtype(args.core, store_dtype),
         fp8_obs=args.fp8_obs,
     )
     fill_replay_synthetic(replay, spec, cfg, min(2048, cfg.replay.capacity),

@@ -45,7 +45,7 @@ from typing import Dict, Optional
 import torch
 
 from .config import Config
-from .models import make_models
+from .models import make_models, state_dtype
 from .ops.polyak import PolyakUpdater
 from .ops.lstm import _FusedLSTMSeq, lstm_seq_pair, lstm_seq_pair_halfgrad
 from .ops.td import td_targets_and_priorities
@@ -199,7 +199,7 @@ class Learner:
         done = batch["done"]                                       # [B, L] fp32
         weight = batch["weight"]                                   # [B] fp32
         # [B, 4, H]; the gated core's state stays in 32 bits
-        st = batch["state"].to(self.dtype if self._lstm else torch.float32)
+        st = batch["state"].to(state_dtype(self.cfg.model.core, self.dtype))
         h_a, c_a = st[:, 0].contiguous(), st[:, 1].contiguous()
         h_c, c_c = st[:, 2].contiguous(), st[:, 3].contiguous()
         length = batch.get("length")

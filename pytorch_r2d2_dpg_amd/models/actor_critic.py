@@ -81,6 +81,12 @@ class _TrunkEncoder(nn.Module):
 CORES = {"lstm": FusedLSTM, "gated": GatedCore}
 
 
+def state_dtype(core: str, dtype: torch.dtype) -> torch.dtype:
+    """What a core of parameters of ``dtype`` takes and stores its recurrent state in:
+    the LSTM's is of that type, the gated core's has 32 bits at least."""
+    return dtype if core == "lstm" else torch.promote_types(dtype, torch.float32)
+
+
 class _Recurrent(nn.Module):
     """The recurrent core of a net, by its name: ``lstm`` or ``gated``."""
 

@@ -21,6 +21,7 @@ from .checkpoint import load_checkpoint, save_checkpoint
 from .config import Config
 from .envs import make_env
 from .learner import Learner
+from .models import state_dtype
 from .parallel.actor_pool import ActorPool
 from .parallel.dist import DistContext
 from .replay.gpu_buffer import GpuSequenceReplay
@@ -47,13 +48,14 @@ def run_training(cfg: Config, device: Optional[str] = None, resume: Optional[str
 
     spec = make_env(cfg.env.name).spec
     R = cfg.replay
+    store_dtype = torch.bfloat16 if cfg.model.dtype == "bf16" else torch.float32
     replay = GpuSequenceReplay(
         capacity=R.capacity, stored_len=R.seq_len + R.n_step,
         obs_shape=spec.obs_shape, action_dim=spec.action_dim,
         hidden_size=cfg.model.hidden_size, per_alpha=R.per_alpha, per_beta=R.per_beta,
         device=device, fp8_obs=R.fp8_obs, seed=cfg.learner.seed + 1000 * rank,
         obs_dtype=torch.uint8 if spec.pixel else torch.float32,
-        store_dtype=torch.bfloat16 if cfg.model.dtype == "bf16" else torch.float32,
+        store_dtype=store_dtype, state_dtype=state_dtype(cfg.model.core, store_dtype),
     )
     learner = Learner(cfg, spec, device=device, dist=dist, replay=replay)
     if resume:

@@ -15,7 +15,7 @@ especially); decode happens inside the fused gather.
 
 from __future__ import annotations
 
-from typing import Dict
+from typing import Dict, Optional
 
 import numpy as np
 import torch
@@ -45,6 +45,7 @@ class GpuSequenceReplay:
         fp8_obs: bool = False,
         store_dtype: torch.dtype = torch.float32,  # action/state (and float obs)
         seed: int = 0,
+        state_dtype: Optional[torch.dtype] = None,  # recurrent state; None: store_dtype
     ):
         self.capacity = capacity
         self.cap2 = _pow2(capacity)
@@ -70,7 +71,7 @@ class GpuSequenceReplay:
                                   device=self.device)
         self.reward = torch.zeros((capacity, L), dtype=torch.float32, device=self.device)
         self.done = torch.zeros((capacity, L), dtype=torch.float32, device=self.device)
-        self.state = torch.zeros((capacity, 4, hidden_size), dtype=store_dtype,
+        self.state = torch.zeros((capacity, 4, hidden_size), dtype=state_dtype or store_dtype,
                                  device=self.device)
         self.length = torch.full((capacity,), stored_len, dtype=torch.int32,
                                  device=self.device)

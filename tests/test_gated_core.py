@@ -182,3 +182,35 @@ def test_learner_graph_replays_match_eager():
         assert abs(a.actor_loss - b.actor_loss) <= 1e-3 * abs(b.actor_loss) + 1e-6
         for p, q in zip(graphed.critic.parameters(), eager.critic.parameters()):
             assert torch.allclose(p.float(), q.float(), atol=2e-3, rtol=1e-2)
+
+
+# ------------------------------------------------ the state on its way to the learner
+@pytest.mark.parametrize("core, stored", [("gated", torch.float32), ("lstm", torch.bfloat16)])
+def test_replay_keeps_the_state_as_wide_as_the_core(core, stored):
+    """The gated core's state stays in 32 bits in a bf16 run's shard too; the LSTM's is
+    bf16 in its learner and may be stored so."""
+    from pytorch_r2d2_dpg_amd.orchestrator import run_training
+    cfg = small_cfg(dtype="bf16", core=core)
+    cfg.actor.num_actors = 1
+    lrn = run_training(cfg, device="cpu", max_steps=1)
+    rep = lrn.replay
+    assert rep.state.dtype == stored and rep.action.dtype == torch.bfloat16
+    state = rep.state[:len(rep)].float()
+    assert torch.equal(state, state.bfloat16().float()) == (stored == torch.bfloat16)
+    assert rep.sample(4)["state"].dtype == stored
+
+
+def test_bench_keeps_the_state_as_wide_as_the_core(monkeypatch, capsys):
+    import sys
+
+    import bench
+    shards = []
+    make = bench.GpuSequenceReplay
+    monkeypatch.setattr(bench, "GpuSequenceReplay", lambda **kw: shards.append(make(**kw)) or shards[-1])
+    for core, stored in (("gated", torch.float32), ("lstm", torch.bfloat16)):
+        monkeypatch.setattr(sys, "argv", [
+            "bench.py", "--device", "cpu", "--core", core, "--hidden", "16", "--batch", "4", "--seq-len", "8",
+            "--burn-in", "2", "--replay-capacity", "16", "--steps", "1", "--warmup", "0"])
+        assert bench.main() in (0, None)
+        assert shards[-1].state.dtype == stored
+    assert capsys.readouterr().out.count('"metric"') == 2
