@@ -81,17 +81,19 @@ OptTensor contiguous(const OptTensor& t) {
     return t ? OptTensor(t->contiguous()) : t;
 }
 
-// A leaf whose gradient accumulator was made by a graph that still lives keeps
-// that graph's stream. Where that is not a stream of the capture, a captured
-// backward pass would wait on a stream outside of the capture, which ends the
-// process. Refused here, while the forward pass is being captured.
+// An input that an eager graph computed, or a leaf whose gradient accumulator was
+// made by an eager graph that still lives, hands its gradient to a node that keeps
+// that graph's stream. Where that is not a stream of the capture, a captured backward
+// pass would wait on a stream outside of the capture, which ends the process. Refused
+// here, while the forward pass is being captured.
 void check_capture(std::initializer_list<OptTensor> inputs) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     (void)hipStreamIsCapturing(stream(), &status);
     if (status == hipStreamCaptureStatusNone) return;
     for (const auto& t : inputs) {
-        if (!t || !t->is_leaf() || !t->requires_grad()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!t || !t->requires_grad()) continue;
+        const auto node = t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t)
+                                       : t->grad_fn();
         if (!node) continue;
         const auto made_on = node->stream();
         if (!made_on) continue;
@@ -102,8 +104,9 @@ void check_capture(std::initializer_list<OptTensor> inputs) {
             outside = status == hipStreamCaptureStatusNone;
         }
         TORCH_CHECK(!outside,
-                    "an eager graph of a leaf that this capture differentiates is alive: delete "
-                    "its outputs (or detach them) before the capture");
+                    "an eager graph of an input that this capture differentiates is alive: delete "
+                    "its outputs (or detach them) before the capture, and compute inputs that "
+                    "are no leaves within it");
     }
 }
 
@@ -136,7 +139,7 @@ void check_modes(const T&... t) {
                                     "no forward-mode derivatives: use the reference on CPU");
 }
 
-// Whether a gradient may be asked for: then the leaves are looked at too.
+// Whether a gradient may be asked for: then a capture's inputs are looked at too.
 template <typename... T>
 bool tracked(const T&... t) {
     if (!torch::GradMode::is_enabled()) return false;

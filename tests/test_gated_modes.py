@@ -156,3 +156,48 @@ def test_recording_the_backward_pass_is_refused(before):
         with pytest.raises(NotImplementedError, match="recorded"):
             back(dy)
         assert torch.autograd.grad(y, x, dy)[0].isfinite().all()
+
+
+# -------------------------------------------------------------------- captures
+@pytest.mark.gpu
+def test_capture_of_an_eagerly_computed_input_is_refused():
+    """Its backward pass would leave the capture for the stream of the eager one."""
+    for x, _, op in args("cuda"):
+        leaf = x.clone().requires_grad_(True)
+        y = leaf * 2
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                op(y)
+        want = torch.autograd.grad(op(y), leaf, torch.ones_like(op(x)))[0]  # eager: as ever
+        assert want.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_capture_of_inputs_computed_within_it():
+    for x, _, op in args("cuda"):
+        leaf = x.clone().requires_grad_(True)
+        dy = torch.randn_like(op(x))
+
+        def step():
+            return torch.autograd.grad(op(leaf * 2), leaf, dy)[0]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        for turn in range(3):
+            with torch.no_grad():
+                leaf.copy_(torch.randn_like(x))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, step())
+        eager = x.clone().requires_grad_(True) * 2
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph), torch.no_grad():  # nothing to differentiate
+            y = op(eager)
+        graph.replay()
+        assert torch.equal(y, op(eager).detach())
