@@ -43,6 +43,7 @@ extern "C" int launch_recurrence_bwd(int, const void*, const float*, const int*,
                                      hipStream_t);
 extern "C" int launch_gated_linear_fwd(int, const void*, const void*, const void*, void*, int,
                                        int, int, hipStream_t);
+extern "C" void gated_linear_cut(int, int, int, int, int, int*, int*, int*);
 extern "C" int gated_linear_bias_parts(int, int, int, int);
 extern "C" int64_t gated_linear_split_sums(int, int, int, int, int, int);
 extern "C" int launch_gated_linear_bwd(int, const void*, const void*, const void*, const void*,
@@ -454,6 +455,16 @@ Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
     return y;
 }
 
+// (tile's rows, tile's columns, splits) of the products that make y and dp, dx, and dw.
+std::vector<std::tuple<int, int, int>> gated_linear_cuts(bool half, int M, int K, int F) {
+    std::vector<std::tuple<int, int, int>> cuts(3);
+    for (int i = 0; i < 3; ++i) {
+        auto& [bm, bn, splits] = cuts[i];
+        gated_linear_cut(half, i, M, K, F, &bm, &bn, &splits);
+    }
+    return cuts;
+}
+
 }  // namespace
 
 void bind_gated(py::module_& m) {
@@ -463,4 +474,7 @@ void bind_gated(py::module_& m) {
           py::arg("gates"), py::arg("h0"), py::arg("lengths"));
     m.def("gated_linear", &gated_linear, "gated linear unit (K11)", py::arg("x"),
           py::arg("weight"), py::arg("bias"));
+    m.def("gated_linear_cuts", &gated_linear_cuts,
+          "(tile rows, tile columns, splits) of K11's products for y and dp, dx, dw",
+          py::arg("bf16"), py::arg("M"), py::arg("K"), py::arg("F"));
 }

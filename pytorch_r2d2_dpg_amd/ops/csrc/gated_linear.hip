@@ -820,6 +820,19 @@ extern "C" int launch_gated_linear_fwd(int is_bf16, const void* x, const void* w
                    : fwd<float>(x, w, bias, y, M, K, F, st);
 }
 
+// How the product `which` is cut: 0 y's and dp's, 1 dx's, 2 dw's.
+extern "C" void gated_linear_cut(int is_bf16, int which, int M, int K, int F, int* bm, int* bn,
+                                 int* splits) {
+    const auto of = [&](auto e) {
+        using E = decltype(e);
+        return which == 0 ? cut_gated<E>(M, K, F) : which == 1 ? cut_dx<E>(M, K, F) : cut_dw<E>(M, K, F);
+    };
+    const Cut cut = is_bf16 ? of(bf16()) : of(float());
+    *bm = cut.bm;
+    *bn = cut.bn;
+    *splits = cut.splits;
+}
+
 extern "C" int gated_linear_bias_parts(int is_bf16, int M, int K, int F) {
     return is_bf16 ? bias_parts<bf16>(M, K, F) : bias_parts<float>(M, K, F);
 }

@@ -322,6 +322,7 @@ def test_linear_larger(M, K, F, dtype):
 
 # every tile that the four products are cut into, whole and past its edges, with
 # and without splits, in 16-byte pieces and element by element
+# (as far as these sizes reach: test_gated_cuts.py has one for every kernel)
 @pytest.mark.parametrize("M, K, F", [
     (4096, 2048, 4096), (5000, 1048, 2056), (5001, 1043, 2055), (8200, 1032, 2056), (8201, 1029, 2054),
     (10240, 1024, 2048), (16384, 520, 136), (16380, 517, 129), (1500, 136, 2048), (1501, 203, 2045),
