@@ -11,16 +11,19 @@
 // activation, the product and (backward) dp are written from the accumulators.
 // The backward pass computes g and u again in place of keeping them: nothing
 // but the inputs lives between the passes, and g and u are never rounded. dp is
-// rounded to the type, as the matrix instructions of the next products take it.
+// rounded to the type, as the matrix instructions of the next products take it: in
+// bf16 a second rounding of half a step behind dx and dW, whose error (of the norm,
+// against 64 bits) is 0.0023 with it and 0.0017 without. db sums dp unrounded.
 //
-// Bound by the matrix instructions where the sizes are large: 16384 x 2048 x 4096
-// (M, K, F) in bf16 takes 436 us forward, and 530, 437 and 430 for dp, dx and dW
-// on the MI355X, 1260, 1040, 1260 and 1280 TFLOP/s, where a library's plain product
-// of 8192^3 reaches 1358; without loads the instructions alone take 254. What is
-// left goes to LDS and, for dp, which reads dy and writes 2F columns, to the memory
-// at the end of each tile. fp32 4000 x 2000 x 4000 takes 950 us a product, 135 of
-// 153 TFLOP/s. Keeping g and u would save the second of the four products and cost
-// 2F columns of 32 bits in memory, 537 MB at the large size: it was not taken.
+// Bound by the matrix instructions where the sizes are large: in a training pass
+// 16384 x 2048 x 4096 (M, K, F) in bf16 takes 471 us forward, and 526, 437 and 411
+// for dp, dx and dW on the MI355X (rocprofv3, medians), 1170, 1050, 1260 and 1340
+// TFLOP/s, where a library's plain product of 8192^3 reaches 1358. What is left goes
+// to LDS and, for dp, which reads dy and writes 2F columns, to the memory at the end
+// of each tile, and to the 23 registers a thread that its largest tile's end spills.
+// fp32 4000 x 2000 x 4000 takes 920 to 958 us a product, 134 to 139 of 153 TFLOP/s.
+// Keeping g and u would save the second of the four products and cost 2F columns of
+// 32 bits in memory, 537 MB at the large size: it was not taken.
 
 #include "gated_common.h"
 
@@ -250,10 +253,11 @@ DEV_INLINE void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
 }
 
 // BM x BN of a result by WM x WN waves, with STAGES of the operands in LDS, of 64
-// bytes a row. A fifth one fits with the largest tile (16384 x 2048 x 4096: 436 us,
-// 457 with two stages of 128 bytes) and with four blocks of the smallest, whose few
-// rows wait for the weights from memory (16 x 2048 x 4096: 11.5 us, 15.2 with four);
-// between them it gained nothing.
+// bytes a row. A fifth one fits with the largest tile and with four blocks of the
+// smallest, whose few rows wait for the weights from memory. Side by side when it was
+// chosen, each kernel alone in a loop: 16384 x 2048 x 4096 forward 436 us, 457 with two
+// stages of 128 bytes; 16 x 2048 x 4096 11.5 us, 15.2 with four stages. Between these
+// tiles it gained nothing.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_ = 4>
 struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
@@ -572,7 +576,8 @@ struct Splits {
     // Groups of a block's threads, which add every GROUPS-th split of the same
     // results. Four where the results are few and their splits many: 128 x 64 of 64
     // splits take 10 us with the product, 18 with one group, but 2048 x 512 of 8
-    // take 58 in place of 55.
+    // take 58 in place of 55. The border lies between these two, which alone were
+    // measured.
     __host__ __device__ bool grouped() const { return splits >= 8 && n <= 1 << 19; }
     int blocks() const {
         const int each = grouped() ? 1024 : 4096;
@@ -634,7 +639,8 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // The tiles that a product may be cut into: how many blocks of one share a CU,
 // what the CU reaches with them in a long product (TFLOP/s), and the time that
 // one block alone takes for a step of DEPTH, which it spends waiting (us); all
-// measured.
+// measured with stages that go straight to LDS. By way of registers a product takes
+// up to half as long again as they say.
 struct Rate {
     int blocks;
     double tflops, alone;

@@ -14,10 +14,9 @@
 // 30 us backward on the MI355X, 4.5 and 5.1 TB/s, where a copy of 2 GiB reaches
 // 4.9. Where the channels are too few to fill the card, time is split over blocks
 // as well: one launch reduces each segment to its map, and the next walks. The
-// gates are read twice then: 16384 steps of 4 rows take 41 + 57 and 49 + 94 us.
-// Blocks that wait for each other's states could read them once, but would join
-// them in the order in which they arrive, and the result would change from run
-// to run.
+// gates are read twice then: 16384 steps of 4 rows take 40 + 57 and 49 + 95 us.
+// Blocks that wait for the maps of the segments before theirs, and join them in
+// their fixed order, could read them once; that is not done.
 //
 // The forward pass keeps the state that each chunk starts from, in 32 bits,
 // 1/CHUNK of the steps: the backward pass walks the chunk again from it in
@@ -421,7 +420,8 @@ recurrence_bwd_kernel(Args<E> p) {
 // of 200 steps 16 and 26 with 7, 20 and 32 with 4. Where 8 waves leave the card
 // half empty and take three passes or more, the chunks are dealt out to
 // `segments` blocks of 4 waves: 64 tiles of 256 steps take 11 and 17 us in 8
-// segments, 15 and 23 in one; of 128 steps 9 and 13 either way.
+// segments, 15 and 23 in one; of 128 steps 9 and 13 either way. These were even H;
+// the rule is the same for odd ones, whose lanes take two loads a pair.
 struct Plan {
     int waves, segments, passes;
 };

@@ -6,9 +6,14 @@
 //
 // Memory bound: about ten operations an element. A row lives in the registers
 // of its threads between the sums over it, so each input is read once. bf16 with a
-// residual, on the MI355X: 32768 rows of 4096 take 182 us forward, 278 backward
-// and 8 for the weight's sums, 5.9 and 4.8 TB/s, where a copy of 2 GiB reaches
-// 4.9; 20480 rows of 512, which the last level of cache holds, 16, 22 and 4 us.
+// residual, on the MI355X: 32768 rows of 4096 take 183 us forward, 277 backward
+// and 8 for the weight's sums, 5.9 and 4.9 TB/s, where a copy of 2 GiB reaches
+// 4.9; 20480 rows of 512, which the last level of cache holds, 17, 22 and 4 us.
+// Rows outside of 256 to 8192 elements are far from that: those of up to 256 leave
+// lanes of their wave idle (1048576 of 64: 283 and 703 us, 1.9 and 0.95 TB/s), those
+// past 8192, and those shorter than a load, are read element by element and three
+// times (16384 of 8192: 184, 294 and 13 us; of 8200: 491, 1174 and 245; 4300000 of 3
+// without a residual: 802, 1123 and 2592).
 
 #include "gated_common.h"
 
@@ -353,7 +358,9 @@ column_sum_kernel(const float* __restrict__ part, E* __restrict__ out, int rows,
 
 // By the runs of a row, the smallest group of threads that holds it with two
 // runs a thread: in bf16 more leave the registers of one wave a SIMD. 0 threads:
-// longer than 8192 elements, or shorter than a run.
+// longer than 8192 elements, or shorter than a run. 512 threads end there in bf16;
+// fp32, whose runs are half as long, takes four of them to the same length. No
+// shape of 1024 threads, which would go on to 16384, has been built.
 struct Shape {
     int threads, runs;
 };
