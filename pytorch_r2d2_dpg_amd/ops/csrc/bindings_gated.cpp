@@ -84,9 +84,10 @@ OptTensor contiguous(const OptTensor& t) {
 
 // An input that an eager graph computed, or a leaf whose gradient accumulator was
 // made by an eager graph that still lives, hands its gradient to a node that keeps
-// that graph's stream. Where that is not a stream of the capture, a captured backward
-// pass would wait on a stream outside of the capture, which ends the process. Refused
-// here, while the forward pass is being captured.
+// that graph's stream. Another stream joins a capture when it waits for one of its
+// events, as a captured backward pass has it do, and is waited for at the pass's end;
+// the default stream cannot, which ends the process. Refused here, while the forward
+// pass is being captured.
 void check_capture(std::initializer_list<OptTensor> inputs) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     (void)hipStreamIsCapturing(stream(), &status);
@@ -97,17 +98,10 @@ void check_capture(std::initializer_list<OptTensor> inputs) {
                                        : t->grad_fn();
         if (!node) continue;
         const auto made_on = node->stream();
-        if (!made_on) continue;
-        bool outside = made_on->id() == 0;  // the default stream is never captured
-        if (!outside) {
-            const at::hip::HIPStream made(at::hip::HIPStream::UNCHECKED, *made_on);
-            (void)hipStreamIsCapturing(made.stream(), &status);
-            outside = status == hipStreamCaptureStatusNone;
-        }
-        TORCH_CHECK(!outside,
-                    "an eager graph of an input that this capture differentiates is alive: delete "
-                    "its outputs (or detach them) before the capture, and compute inputs that "
-                    "are no leaves within it");
+        TORCH_CHECK(!made_on || made_on->id() != 0,
+                    "an eager graph of an input that this capture differentiates is alive on the "
+                    "default stream: delete its outputs (or detach them) before the capture, and "
+                    "compute inputs that are no leaves within it");
     }
 }
 

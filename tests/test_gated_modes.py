@@ -201,3 +201,63 @@ def test_capture_of_inputs_computed_within_it():
             y = op(eager)
         graph.replay()
         assert torch.equal(y, op(eager).detach())
+
+
+@pytest.mark.gpu
+def test_capture_over_an_eager_graph_of_a_side_stream():
+    """A side stream joins the capture, unlike the default stream: a warm-up's graph may live."""
+    for x, _, op in args("cuda"):
+        leaf = x.clone().requires_grad_(True)
+        dy = torch.randn_like(op(x))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            alive = op(leaf)
+            torch.autograd.grad(alive, leaf, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = op(leaf)
+            got = torch.autograd.grad(y, leaf, dy)[0]
+        y = y.detach()
+        for _ in range(3):
+            with torch.no_grad():
+                leaf.copy_(torch.randn_like(x))
+            graph.replay()
+            torch.cuda.synchronize()
+            fresh = leaf.detach().clone().requires_grad_(True)
+            want = op(fresh)
+            assert torch.equal(y, want) and torch.equal(got, torch.autograd.grad(want, fresh, dy)[0])
+        del alive
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_graphed_callables(dtype):
+    """torch's own capture of a module, forward and backward, whose warm-up graph lives."""
+    from pytorch_r2d2_dpg_amd.models import GatedCore
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.core = GatedCore(24, 32)
+
+        def forward(self, x):
+            return self.core(x)[0]
+
+    torch.manual_seed(6)
+    net = Net().to("cuda", dtype)
+    plain = Net().to("cuda", dtype)
+    plain.load_state_dict(net.state_dict())
+    sample = torch.randn(9, 4, 24, device="cuda", dtype=dtype, requires_grad=True)
+    graphed = torch.cuda.make_graphed_callables(net, (sample,))
+    for _ in range(3):
+        x = torch.randn(9, 4, 24, device="cuda", dtype=dtype, requires_grad=True)
+        dy = torch.randn(9, 4, 32, device="cuda", dtype=dtype)
+        want = torch.autograd.grad(plain(x), [x, *plain.parameters()], dy)
+        got = torch.autograd.grad(graphed(x), [x, *net.parameters()], dy)
+        # Library products may sum in another order: as in test_gated_core.py either side
+        # is 24 roundings of half a step off at most.
+        for a, b in zip(got, want):
+            assert (a - b).double().norm() <= 24 * torch.finfo(dtype).eps * b.double().norm()
