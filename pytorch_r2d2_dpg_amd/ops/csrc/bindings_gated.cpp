@@ -119,19 +119,26 @@ bool recorded() {
            Modes::get_mode(Mode::FUNCTIONAL);
 }
 
-// What a launch that torch's dispatcher does not see cannot serve: a recording, and
-// tangents, which the kernels would drop. Forward mode has a switch of its own:
-// inference mode turns it off, no_grad does not. Both passes look: a recording or a
-// tangent may begin with the outputs' gradients.
+// What a launch that torch's dispatcher does not see cannot serve: a recording, tensors
+// without memory (a fake one that outlived its mode has a null pointer and is on GPU by
+// its own account), and tangents, which the kernels would drop. Forward mode has a
+// switch of its own: inference mode turns it off, no_grad does not. Both passes look: a
+// recording or a tangent may begin with the outputs' gradients.
 template <typename... T>
 void check_modes(const T&... t) {
     TORCH_CHECK_NOT_IMPLEMENTED(!recorded(), "the kernels' launches cannot be recorded (traced, "
                                              "exported or run on fake tensors): use the "
                                              "reference on CPU");
-    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-    for (const auto& v : std::initializer_list<OptTensor>{t...})
-        TORCH_CHECK_NOT_IMPLEMENTED(!v || !v->defined() || !v->_fw_grad(0).defined(),
+    const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const auto& v : std::initializer_list<OptTensor>{t...}) {
+        if (!v || !v->defined()) continue;
+        TORCH_CHECK_NOT_IMPLEMENTED(
+            v->has_storage() && (v->numel() == 0 || v->storage().data() != nullptr),
+            "a tensor without memory (fake, wrapped by a transform, or a zero that is only said "
+            "to be one) has nothing for a kernel to read");
+        TORCH_CHECK_NOT_IMPLEMENTED(!forward || !v->_fw_grad(0).defined(),
                                     "no forward-mode derivatives: use the reference on CPU");
+    }
 }
 
 // Whether a gradient may be asked for: then a capture's inputs are looked at too.
@@ -323,7 +330,7 @@ struct GatedRecurrenceBackward : Node {
 
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const OptTensor& h0,
                                             const OptTensor& lengths) {
-    check_modes(gates, h0);
+    check_modes(gates, h0, lengths);
     check_first(gates, "gates");
     const c10::DeviceGuard guard(gates.device());
     TORCH_CHECK_VALUE(gates.dim() == 3 && gates.size(2) % 3 == 0,

@@ -261,3 +261,32 @@ def test_graphed_callables(dtype):
         # is 24 roundings of half a step off at most.
         for a, b in zip(got, want):
             assert (a - b).double().norm() <= 24 * torch.finfo(dtype).eps * b.double().norm()
+
+
+# --------------------------------------------------------- tensors without memory
+@built
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_tensors_without_memory_are_refused(device):
+    """Fake tensors that outlive their mode, and zeros that are only said to be: their
+    pointer is null. No GPU takes part: refused before the device is looked for."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w, w2 = (torch.empty(*s, device=device) for s in ((3, 8), (8,), (6, 8)))
+        g, h0 = torch.empty(2, 3, 6, device=device), torch.empty(3, 2, device=device)
+        n = torch.empty(3, dtype=torch.int32, device=device)
+    e = hip_ext()
+    calls = [lambda: e.layer_norm(x, w, None, 1e-5, None), lambda: e.gated_recurrence(g, None, None),
+             lambda: e.gated_linear(x, w2, None)]
+    if device == "cuda":
+        calls += [lambda: layer_norm(x, w), lambda: gated_recurrence(g), lambda: gated_linear(x, w2)]
+    else:  # in any place
+        real, rg, zero = torch.randn(3, 8), torch.randn(2, 3, 6), torch._efficientzerotensor((3, 8))
+        calls += [lambda: e.layer_norm(real, w, None, 1e-5, None),
+                  lambda: e.layer_norm(real, torch.ones(8), w, 1e-5, None),
+                  lambda: e.layer_norm(real, torch.ones(8), None, 1e-5, zero),
+                  lambda: e.layer_norm(zero, torch.ones(8), None, 1e-5, None),
+                  lambda: e.gated_recurrence(rg, h0, None), lambda: e.gated_recurrence(rg, None, n),
+                  lambda: e.gated_linear(real, w2, None), lambda: e.gated_linear(zero, torch.ones(6, 8), None)]
+    for call in calls:
+        with pytest.raises(NotImplementedError, match="memory"):
+            call()
