@@ -78,9 +78,9 @@ void check(const Tensor& t, const char* name, const Tensor& first, torch::Scalar
     TORCH_CHECK(t.device() == first.device(), name, " must be on ", first.device());
 }
 
-OptTensor contiguous(const OptTensor& t) {
-    return t ? OptTensor(t->contiguous()) : t;
-}
+// The values as they lie in the kernels' order, with a sign that is only noted applied.
+Tensor contiguous(const Tensor& t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+OptTensor contiguous(const OptTensor& t) { return t ? OptTensor(contiguous(*t)) : t; }
 
 // An input that an eager graph computed, or a leaf whose gradient accumulator was
 // made by an eager graph that still lives, hands its gradient to a node that keeps
@@ -230,9 +230,9 @@ struct LayerNormBackward : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         const Tensor in = x.unpack();
         const OptTensor res = optional(residual);
-        const Tensor dy = grads[0].defined() ? grads[0].contiguous() : torch::zeros_like(in);
+        const Tensor dy = grads[0].defined() ? contiguous(grads[0]) : torch::zeros_like(in);
         OptTensor ds;
-        if (res && grads[1].defined()) ds = grads[1].contiguous();
+        if (res && grads[1].defined()) ds = contiguous(grads[1]);
         auto [dx, dwb] = layer_norm_bwd(in, res, weight.unpack(), dy, ds, eps);
         return once({dx, should_compute_output(1) ? dwb[0] : Tensor(),
                      should_compute_output(2) ? dwb[1] : Tensor(), res ? dx : Tensor()},
@@ -253,7 +253,7 @@ variable_list layer_norm(const Tensor& x, const Tensor& weight, const OptTensor&
     if (bias) check(*bias, "bias", x, x.scalar_type(), {dim});
     if (residual) check(*residual, "residual", x, x.scalar_type(), x.sizes());
     const bool track = tracked(x, weight, bias, residual);
-    const Tensor in = x.contiguous(), w = weight.contiguous();
+    const Tensor in = contiguous(x), w = contiguous(weight);
     const OptTensor b = contiguous(bias), r = contiguous(residual);
     auto [y, s] = layer_norm_fwd(in, w, b, r, eps);
     if (track) {
@@ -319,10 +319,10 @@ struct GatedRecurrenceBackward : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         const Tensor g = gates.unpack();
         const Tensor dy = grads[0].defined()
-            ? grads[0].contiguous()
+            ? contiguous(grads[0])
             : torch::zeros({g.size(0), g.size(1), g.size(2) / 3}, g.options());
         OptTensor dhT;
-        if (grads[1].defined()) dhT = grads[1].contiguous();
+        if (grads[1].defined()) dhT = contiguous(grads[1]);
         auto [dgates, dh0] = gated_recurrence_bwd(g, kept.unpack(), optional(lengths), dy, dhT);
         return once({dgates, should_compute_output(1) ? dh0 : Tensor()}, "gated_recurrence");
     }
@@ -342,7 +342,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, const OptTensor
     if (h0) check(*h0, "h0 (the state is not rounded)", gates, torch::kFloat32, {B, H});
     if (lengths) check(*lengths, "lengths", gates, torch::kInt32, {B});
     const bool track = tracked(gates, h0);
-    const Tensor g = gates.contiguous();
+    const Tensor g = contiguous(gates);
     const OptTensor h = contiguous(h0), n = contiguous(lengths);
     auto [y, hT, kept] = gated_recurrence_fwd(g, h, n, track);
     if (track) {
@@ -416,7 +416,7 @@ struct GatedLinearBackward : Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         return once(gated_linear_bwd(x.unpack(), weight.unpack(), optional(bias),
-                                     grads[0].contiguous(), should_compute_output(0),
+                                     contiguous(grads[0]), should_compute_output(0),
                                      should_compute_output(1), should_compute_output(2)),
                     "gated_linear");
     }
@@ -443,7 +443,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
     // row and its value's
     TORCH_CHECK((F + 256) * K <= MOST && 512 * F <= MOST, "weight is too large");
     const bool track = tracked(x, weight, bias);
-    const Tensor in = x.contiguous(), w = weight.contiguous();
+    const Tensor in = contiguous(x), w = contiguous(weight);
     const OptTensor b = contiguous(bias);
     auto y = gated_linear_fwd(in, w, b);
     if (track) {

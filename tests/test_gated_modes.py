@@ -290,3 +290,31 @@ def test_tensors_without_memory_are_refused(device):
     for call in calls:
         with pytest.raises(NotImplementedError, match="memory"):
             call()
+
+
+@pytest.mark.gpu
+def test_negations_that_are_only_noted():
+    """Such as the imaginary part of a conjugate: memory holds the values before the sign."""
+    def neg(t):
+        return torch._neg_view(t)
+
+    x, w, g, h0, w2, r = (torch.randn(*s, device="cuda") for s in
+                          ((3, 8), (8,), (2, 3, 6), (3, 2), (6, 8), (3, 8)))
+    for op, ts in ((lambda a, b, c: layer_norm(a, b, b, residual=c)[0], (x, w, r)),
+                   (lambda a, b: gated_recurrence(a, b)[0], (g, h0)),
+                   (lambda a, b: gated_linear(a, b), (x, w2))):
+        assert torch.equal(op(*map(neg, ts)), op(*(-t for t in ts)))
+        leaves = [t.clone().requires_grad_(True) for t in ts]
+        y = op(*map(neg, leaves))
+        dy = torch.randn_like(y)
+        got = torch.autograd.grad(y, leaves, neg(dy))
+        plain = [(-t).detach().requires_grad_(True) for t in ts]
+        for a, b in zip(got, torch.autograd.grad(op(*plain), plain, dy)):  # the signs cancel
+            assert torch.equal(a, b)
+    z = torch.complex(torch.randn(1, 1, device="cuda"), torch.randn(1, 1, device="cuda"))
+    one, bias = torch.ones(1, device="cuda"), torch.ones(2, device="cuda")
+    im = z.conj().imag
+    assert im.is_neg() and im.is_contiguous()
+    ww = torch.ones(2, 1, device="cuda")
+    assert torch.equal(gated_linear(im, ww, bias), gated_linear(-z.imag, ww, bias))
+    assert torch.equal(layer_norm(one, one, im[0]), layer_norm(one, one, -z.imag[0]))
